@@ -5,6 +5,7 @@ path it covers; use ``import deepgemm_b200 as deep_gemm``. Every operator calls 
 (include/dgb200.h); there is no CPU or PyTorch fallback.
 """
 from . import _lib, testing, utils  # noqa: F401
+from .activation import swiglu, swiglu_backward, swiglu_per_token_cast_to_fp8  # noqa: F401
 from .bf16 import (  # noqa: F401
     bf16_gemm_nn,
     bf16_gemm_nt,
@@ -53,6 +54,14 @@ from .nvfp4 import (  # noqa: F401
     pack_nvfp4_sf_mn_major,
     per_token_cast_to_nvfp4,
     per_token_cast_to_nvfp4_into,
+)
+from .permute import (  # noqa: F401
+    MoeDispatchPlan,
+    moe_dispatch_plan,
+    moe_permute,
+    moe_permute_backward,
+    moe_unpermute,
+    moe_unpermute_backward,
 )
 from .runtime import (  # noqa: F401
     get_mk_alignment_for_contiguous_layout,

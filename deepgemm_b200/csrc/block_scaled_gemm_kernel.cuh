@@ -1,0 +1,468 @@
+// FP8 GEMM whose operands carry one FP32 scale for every block of 128 (A: 1 x 128, B: 128 x 128):
+//   D[m, n] = C[m, n] + sum over K blocks of  sfa[m, kb] sfb[n / 128, kb] * sum_{k in kb} A[m, k] B[n, k]
+// for the dense, m-grouped (row ids or psum) and masked layouts. The tensor core's block-scaled kinds take power-of-two scales
+// only, so the products of one K block are summed by tcgen05.mma (kind::f8f6f4) into an accumulator of their own in
+// tensor memory, and the epilogue warps keep the running sum in registers: one FP32 multiply-add per element and K block with
+// the product of the two scales. Behavioural counterpart in the reference: its FP32-scale kernel of the previous architecture
+// (deep_gemm/include/deep_gemm/impls/sm90_fp8_gemm_1d2d.cuh), reached there with disable_ue8m0_cast.
+//
+// Warp roles (384 threads): warp 0 loads A tiles, warp 3 B tiles, warp 1 issues the MMAs, warp 2 owns the tensor memory,
+// warps 4-11 add up (TMEM lane quarter = warp index % 4, two warps per quarter split the columns). A thread owns one row's
+// half of the tile in registers, so a scale is one scalar per thread and K block and no value crosses lanes until the store.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "gemm_kernel.cuh"
+#include "ptx.cuh"
+
+namespace dgb {
+
+struct BlockScaledParams {
+    const float* sfa;  // element (group, row, kb) at sfa[group * sfa_group_stride + row * sfa_row_stride + kb * sfa_k_stride]
+    const float* sfb;  // element (group, nb, kb) likewise, nb = n / 128
+    long long sfa_group_stride, sfa_row_stride, sfa_k_stride;
+    long long sfb_group_stride, sfb_n_stride, sfb_k_stride;
+    void* d;
+    const float* c;  // FP32 output only: added to the product; may be d itself
+    long long d_row_stride, c_row_stride;  // elements
+    const int* layout;
+    int mode;  // kModeDense / kModeRowIds / kModePsum / kModeMasked (A and D [G, m, *])
+    int m, n, k, num_groups, alignment, store_padding;
+    int b_mn_major;   // B is [groups, k, n] with n contiguous
+    int a_box_rows;   // rows of A that one load brings: 128, or fewer where no tile has more
+};
+
+// kind::f8f6f4 descriptor: E4M3 operands (format 0), FP32 accumulator.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3_f32(uint32_t m, uint32_t n) {
+    return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tcgen05_mma_f8f6f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tcgen05_mma_f8f6f4_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Tiled 3-D loads (same rules as the 2-D ones): into this CTA's shared memory, completing on its own barrier or on one of the pair's.
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        :: "r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int32_t x, int32_t y,
+                                                 int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        :: "r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+template <int BLOCK_N, int kStages, bool kPair>
+struct BlockScaledSmem {
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = BLOCK_N * 128 / (kPair ? 2 : 1);
+    static constexpr int kOffA = 0;
+    static constexpr int kOffB = kOffA + kStages * kABytes;
+    static constexpr int kOffStage = kOffB + kStages * kBBytes;  // epilogue: 32 rows x 64 bytes per warp
+    static constexpr int kOffBar = kOffStage + 8 * 2048;
+    static constexpr int kNumBars = 2 * kStages + 2 * (512 / (BLOCK_N < 64 ? 64 : BLOCK_N));
+    static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+    static constexpr int kOffGroups = kOffMisc + 16;
+    static constexpr int kTotal = kOffGroups + 3 * kMaxCachedGroups * 4;
+    static constexpr int kDynamicBytes = kTotal + 1024;  // slack to align the base to 1024 B
+};
+
+struct BlockScaledTile {
+    int row0;   // first row of this CTA's 128 in the flattened A / D (masked: inside the group)
+    int rows;   // rows of them to store; may be zero or negative for the second CTA of a pair
+    int group;  // < 0: nothing to do, every role skips the tile
+    int n0;
+};
+
+// Walks the output tiles. Groups come from the table that the prologue puts into shared memory: start row, rows to
+// compute and running tile count of each.
+template <int BLOCK_N, bool kPair>
+struct BlockScaledScheduler {
+    static constexpr int kTileM = kPair ? 256 : 128;
+    const BlockScaledParams& p;
+    const int *start, *rows, *tiles_end;
+    int num_n_blocks, tile, stride, sub, g;
+
+    __device__ BlockScaledScheduler(const BlockScaledParams& params, const int* table)
+        : p(params), start(table), rows(table + kMaxCachedGroups), tiles_end(table + 2 * kMaxCachedGroups),
+          num_n_blocks((params.n + BLOCK_N - 1) / BLOCK_N), tile(static_cast<int>(blockIdx.x) / (kPair ? 2 : 1)),
+          stride(static_cast<int>(gridDim.x) / (kPair ? 2 : 1)), sub(kPair ? static_cast<int>(blockIdx.x & 1) * 128 : 0), g(0) {}
+
+    // Rows of a group from the layout words; whatever they hold, no row at or past p.m is named.
+    __device__ __forceinline__ static void group_extent(const BlockScaledParams& p, int group, int& first, int& count) {
+        if (p.mode == kModeMasked) {
+            first = 0;
+            count = min(max(__ldg(p.layout + group), 0), p.m);
+            return;
+        }
+        const int prev_end = group == 0 ? 0 : min(max(__ldg(p.layout + group - 1), 0), p.m);
+        const int end = min(max(__ldg(p.layout + group), 0), p.m);
+        const long long al = p.alignment;
+        first = static_cast<int>(min((prev_end + al - 1) / al * al, static_cast<long long>(p.m)));
+        const int last = p.store_padding ? static_cast<int>(min((end + al - 1) / al * al, static_cast<long long>(p.m))) : end;
+        count = end > first ? last - first : 0;
+    }
+
+    __device__ bool next(BlockScaledTile& t) {
+        if (p.mode == kModeDense || p.mode == kModeRowIds) {
+            const int num_m_blocks = (p.m + kTileM - 1) / kTileM;
+            if (tile >= num_m_blocks * num_n_blocks) return false;
+            const int nb = tile / num_m_blocks;
+            t.row0 = (tile - nb * num_m_blocks) * kTileM + sub;
+            t.rows = min(128, p.m - t.row0);
+            t.n0 = nb * BLOCK_N;
+            t.group = p.mode == kModeDense ? 0 : __ldg(p.layout + t.row0);  // (no pairs with row ids: t.row0 < p.m)
+            if (t.group >= p.num_groups) {
+                if (threadIdx.x == 0) report_error(kBadArgument, t.row0, t.group);
+                t.group = -1;
+            }
+            tile += stride;
+            return true;
+        }
+        g = group_of_tile(tiles_end, g, p.num_groups, tile);
+        if (g >= p.num_groups) return false;
+        const int local = tile - (g == 0 ? 0 : tiles_end[g - 1]);
+        const int num_m_blocks = (rows[g] + kTileM - 1) / kTileM;
+        const int nb = local / num_m_blocks;
+        const int mb = local - nb * num_m_blocks;
+        t.row0 = start[g] + mb * kTileM + sub;
+        t.rows = min(128, rows[g] - mb * kTileM - sub);
+        t.n0 = nb * BLOCK_N;
+        t.group = g;
+        tile += stride;
+        return true;
+    }
+};
+
+constexpr int kRegsBsControl = 56, kRegsBsSum = 224;  // 128 x 56 + 256 x 224 = 384 x 168, what the block is launched with
+
+template <int BLOCK_N, int kStages, bool kF32, bool kPair>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                                const __grid_constant__ BlockScaledParams p) {
+    using L = BlockScaledSmem<BLOCK_N, kStages, kPair>;
+    using Sched = BlockScaledScheduler<BLOCK_N, kPair>;
+    constexpr int kCtas = kPair ? 2 : 1;
+    constexpr int kAccums = 512 / (BLOCK_N < 64 ? 64 : BLOCK_N);  // accumulators in tensor memory: K blocks in flight
+    constexpr int kCols = BLOCK_N / 2;                            // columns a thread sums
+    static_assert(BLOCK_N == 32 || BLOCK_N == 64 || BLOCK_N == 128 || BLOCK_N == 256, "tile width");
+    static_assert(!kPair || BLOCK_N == 256, "pairs work on 256 x 256 tiles");
+    static_assert(L::kDynamicBytes <= 232448, "shared memory budget");
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+    uint64_t* empty_bar = full_bar + kStages;
+    uint64_t* tmem_full_bar = empty_bar + kStages;
+    uint64_t* tmem_empty_bar = tmem_full_bar + kAccums;
+    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kOffMisc + 4);
+    int* table = reinterpret_cast<int*>(smem + L::kOffGroups);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cta_rank = kPair ? cluster_cta_rank() : 0u;
+    const bool leader_cta = cta_rank == 0;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(full_bar + i, 2 * kCtas);  // the A loader and the B loader of every CTA
+            mbar_init(empty_bar + i, 1);         // tcgen05.commit of the MMA issuer
+        }
+        for (int i = 0; i < kAccums; ++i) {
+            mbar_init(tmem_full_bar + i, 1);
+            mbar_init(tmem_empty_bar + i, 8 * kCtas);  // lane 0 of each summing warp
+        }
+        fence_mbar_init();
+        prefetch_tensormap(&tm_a);
+        prefetch_tensormap(&tm_b);
+    }
+    pdl_prologue();  // everything above touches only this CTA's shared memory and the kernel's own parameters
+    if (p.mode == kModePsum || p.mode == kModeMasked) {
+        int* tiles_end = table + 2 * kMaxCachedGroups;
+        for (int i = threadIdx.x; i < p.num_groups; i += kGemmThreads) {
+            int first, count;
+            Sched::group_extent(p, i, first, count);
+            table[i] = first;
+            table[kMaxCachedGroups + i] = count;
+            tiles_end[i] = (count + Sched::kTileM - 1) / Sched::kTileM * ((p.n + BLOCK_N - 1) / BLOCK_N);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const int chunk = (p.num_groups + 31) / 32;
+            const int lo = min(static_cast<int>(lane) * chunk, p.num_groups), hi = min(lo + chunk, p.num_groups);
+            int sum = 0;
+            for (int i = lo; i < hi; ++i) sum += tiles_end[i];
+            int incl = sum;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, off);
+                if (static_cast<int>(lane) >= off) incl += v;
+            }
+            int run = incl - sum;
+            for (int i = lo; i < hi; ++i) {
+                run += tiles_end[i];
+                tiles_end[i] = run;
+            }
+        }
+    }
+    if constexpr (kPair) cluster_sync_all();  // both CTAs run and see each other's initialised barriers
+    if (warp == 2) {
+        if constexpr (kPair) tmem_alloc_pair(tmem_ptr_smem, 512);
+        else tmem_alloc(tmem_ptr_smem, 512);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if constexpr (kPair) cluster_sync_all();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    const int num_kb = (p.k + 127) / 128;
+
+    // In a pair the leader's loaders announce the bytes of both CTAs (their loads are alike), the other CTA's only arrive.
+    auto stage_arrive = [&](uint32_t stage, uint32_t bytes) {
+        if constexpr (kPair) {
+            if (leader_cta) mbar_arrive_expect_tx(full_bar + stage, 2 * bytes);
+            else mbar_arrive_cluster(map_to_cta(smem_u32(full_bar + stage), 0));
+        } else {
+            mbar_arrive_expect_tx(full_bar + stage, bytes);
+        }
+    };
+    auto load_tile = [&](int smem_off, const CUtensorMap* map, uint32_t stage, int x, int y, int z) {
+        if constexpr (kPair) tma_load_3d_pair(smem + smem_off, map, map_to_cta(smem_u32(full_bar + stage), 0), x, y, z);
+        else tma_load_3d(smem + smem_off, map, full_bar + stage, x, y, z);
+    };
+
+    if (warp < 4) {
+        setmaxnreg_dec<kRegsBsControl>();
+        if (warp == 0 || warp == 3) {
+            // ------------------------------------------------------------ loaders: A (warp 0) and B (warp 3)
+            const bool is_a = warp == 0;
+            const bool elected = elect_one();
+            Sched sched(p, table);
+            BlockScaledTile t;
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            while (ok && sched.next(t)) {
+                if (t.group < 0) continue;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    ok = mbar_wait(empty_bar + stage, phase ^ 1, abort_flag, kTimeoutEmpty, kb);
+                    if (!ok) break;
+                    if (elected) {
+                        if (is_a) {
+                            stage_arrive(stage, static_cast<uint32_t>(p.a_box_rows) * 128);
+                            load_tile(L::kOffA + stage * L::kABytes, &tm_a, stage, kb * 128, t.row0, p.mode == kModeMasked ? t.group : 0);
+                        } else {
+                            stage_arrive(stage, L::kBBytes);
+                            const int off = L::kOffB + stage * L::kBBytes;
+                            const int n = t.n0 + static_cast<int>(cta_rank) * (BLOCK_N / kCtas);  // first channel of this CTA
+                            if (BLOCK_N >= 128 && p.b_mn_major) {
+#pragma unroll
+                                for (int h = 0; h < BLOCK_N / kCtas / 128; ++h)  // boxes of 128 channels x 128 K rows
+                                    load_tile(off + h * 16384, &tm_b, stage, n + h * 128, kb * 128, t.group);
+                            } else {
+                                load_tile(off, &tm_b, stage, kb * 128, n, t.group);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                }
+            }
+        } else if (warp == 1 && leader_cta) {
+            // ------------------------------------------------------------ MMA issuer: one accumulator per K block
+            const bool elected = elect_one();
+            Sched sched(p, table);
+            BlockScaledTile t;
+            uint32_t stage = 0, phase = 0, as = 0, aphase = 0;
+            const bool b_mn = BLOCK_N >= 128 && p.b_mn_major;
+            const uint32_t idesc = make_idesc_e4m3_f32(128 * kCtas, BLOCK_N) | (b_mn ? (1u << 16) : 0u);
+            const uint32_t a_base = smem_u32(smem + L::kOffA), b_base = smem_u32(smem + L::kOffB);
+            const uint32_t b_step = b_mn ? 256u : 2u;  // 32 K rows of 128 bytes, or 32 bytes inside the swizzle span
+            bool ok = true;
+            while (ok && sched.next(t)) {
+                if (t.group < 0) continue;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    ok = mbar_wait(tmem_empty_bar + as, aphase ^ 1, abort_flag, kTimeoutTmemEmpty, kb) &&
+                         mbar_wait(full_bar + stage, phase, abort_flag, kTimeoutFull, kb);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    if (elected) {
+                        const uint64_t adesc = make_kmajor_sw128_desc(a_base + stage * L::kABytes);
+                        const uint64_t bdesc = b_mn ? make_mnmajor_sw128_desc(b_base + stage * L::kBBytes, 16384)
+                                                    : make_kmajor_sw128_desc(b_base + stage * L::kBBytes);
+                        const uint32_t acc = tmem_base + as * (BLOCK_N < 64 ? 64 : BLOCK_N);
+#pragma unroll
+                        for (uint32_t k4 = 0; k4 < 4; ++k4) {
+                            if constexpr (kPair) tcgen05_mma_f8f6f4_pair(acc, adesc + k4 * 2, bdesc + k4 * b_step, idesc, k4);
+                            else tcgen05_mma_f8f6f4(acc, adesc + k4 * 2, bdesc + k4 * b_step, idesc, k4);
+                        }
+                        if constexpr (kPair) {
+                            tcgen05_commit_pair(empty_bar + stage, 3);
+                            tcgen05_commit_pair(tmem_full_bar + as, 3);
+                        } else {
+                            tcgen05_commit(empty_bar + stage);
+                            tcgen05_commit(tmem_full_bar + as);
+                        }
+                    }
+                    __syncwarp();
+                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                    if (++as == kAccums) { as = 0; aphase ^= 1; }
+                }
+            }
+        }
+    } else {
+        setmaxnreg_inc<kRegsBsSum>();
+        // ---------------------------------------------------------------- running sums and epilogue (8 warps)
+        const uint32_t q = warp & 3, half = (warp - 4) >> 2;
+        const int r = static_cast<int>(q * 32 + lane);
+        uint8_t* stage_buf = smem + L::kOffStage + (warp - 4) * 2048;
+        Sched sched(p, table);
+        BlockScaledTile t;
+        uint32_t as = 0, aphase = 0;
+        bool ok = true;
+        while (ok && sched.next(t)) {
+            if (t.group < 0) continue;
+            const bool warp_has_rows = static_cast<int>(q * 32) < t.rows;
+            const int col0 = t.n0 + static_cast<int>(half) * kCols;
+            const long long group = t.group;
+            // rows that are not stored take the scale of the last one that is: never an address outside the tensor
+            const long long sf_row = t.row0 + min(r, max(t.rows - 1, 0));
+            const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + sf_row * p.sfa_row_stride;
+            const float* sfb = p.sfb + group * p.sfb_group_stride + static_cast<long long>(min(col0, p.n - 1) / 128) * p.sfb_n_stride;
+            float acc[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+            // scales two K blocks ahead of their use
+            float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
+            if (warp_has_rows) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (i < num_kb) {
+                        sa[i] = __ldg(sfa + i * p.sfa_k_stride);
+                        sb[i] = __ldg(sfb + i * p.sfb_k_stride);
+                    }
+            }
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const float s = sa[0] * sb[0];
+                sa[0] = sa[1];
+                sb[0] = sb[1];
+                if (warp_has_rows && kb + 2 < num_kb) {
+                    sa[1] = __ldg(sfa + (kb + 2) * p.sfa_k_stride);
+                    sb[1] = __ldg(sfb + (kb + 2) * p.sfb_k_stride);
+                }
+                ok = mbar_wait(tmem_full_bar + as, aphase, abort_flag, kTimeoutTmemFull, kb);
+                if (!ok) break;
+                tcgen05_fence_after();
+                if (warp_has_rows) {
+                    const uint32_t tmem_row = tmem_base + as * (BLOCK_N < 64 ? 64 : BLOCK_N) + ((q * 32u) << 16) + half * kCols;
+                    if constexpr (kCols >= 64) {
+                        uint32_t v[2][32];
+                        tmem_ld_32x32b_x32(tmem_row, v[0]);
+#pragma unroll
+                        for (int c = 0; c < kCols / 32; ++c) {
+                            tmem_ld_wait();
+                            if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(tmem_row + (c + 1) * 32, v[(c + 1) & 1]);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[c * 32 + i]);
+                        }
+                    } else {
+                        uint32_t v[kCols];
+#pragma unroll
+                        for (int c = 0; c < kCols / 16; ++c) tmem_ld_32x32b_x16(tmem_row + c * 16, v + c * 16);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < kCols; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s, acc[i]);
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (leader_cta) mbar_arrive(tmem_empty_bar + as);
+                    else mbar_arrive_cluster(map_to_cta(smem_u32(tmem_empty_bar + as), 0));
+                }
+                if (++as == kAccums) { as = 0; aphase ^= 1; }
+            }
+            if (!ok) break;
+            if (!warp_has_rows) continue;
+            // Store: a slab of 32 rows x 64 bytes at a time is turned through shared memory (16-byte chunks, XOR-swizzled), so that a
+            // store instruction of the warp writes eight rows' 64 contiguous bytes instead of 16 bytes of 32 rows.
+            constexpr int kSlab = kF32 ? 16 : 32;  // columns
+            constexpr int kSlabs = (kCols + kSlab - 1) / kSlab;
+            const long long row_base = (p.mode == kModeMasked ? group * p.m : 0) + t.row0 + static_cast<int>(q * 32);
+            const int rows_here = t.rows - static_cast<int>(q * 32);
+#pragma unroll
+            for (int s = 0; s < kSlabs; ++s) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint4 o;
+                    if constexpr (kF32) {
+                        const float* a = acc + s * kSlab + i * 4;
+                        o = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+                    } else if (s * kSlab + i * 8 < kCols) {
+                        const float* a = acc + s * kSlab + i * 8;
+                        o = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
+                    } else {
+                        o = make_uint4(0, 0, 0, 0);
+                    }
+                    *reinterpret_cast<uint4*>(stage_buf + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = o;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = static_cast<int>(lane >> 2) + 8 * j, chunk = static_cast<int>(lane & 3);
+                    const int in_half = s * kSlab + chunk * (kF32 ? 4 : 8);
+                    const int col = col0 + in_half;
+                    if (row >= rows_here || in_half >= kCols || col >= p.n) continue;  // n is a multiple of 8: a chunk is inside or outside
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage_buf + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+                    const long long at = (row_base + row) * p.d_row_stride + col;
+                    if constexpr (kF32) {
+                        float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+                        if (p.c != nullptr) {
+                            const float4 c4 = *reinterpret_cast<const float4*>(p.c + (row_base + row) * p.c_row_stride + col);
+                            f = make_float4(c4.x + f.x, c4.y + f.y, c4.z + f.z, c4.w + f.w);
+                        }
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at) = f;
+                    } else {
+                        st_global_v4(static_cast<__nv_bfloat16*>(p.d) + at, v.x, v.y, v.z, v.w);
+                    }
+                }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    tcgen05_fence_before();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        // Let copies and MMAs that were already issued land before shared and tensor memory are released.
+        __nanosleep(100000);
+        __syncthreads();
+    }
+    if constexpr (kPair) cluster_sync_all();  // the other CTA may still signal barriers of this one or read its shared memory
+    if (warp == 2) {
+        tcgen05_fence_after();
+        if constexpr (kPair) tmem_dealloc_pair(tmem_base, 512);
+        else tmem_dealloc(tmem_base, 512);
+    }
+}
+
+}  // namespace dgb

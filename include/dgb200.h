@@ -28,6 +28,8 @@ extern "C" {
  * deep_gemm/include/deep_gemm/common/types.cuh:20-28). */
 #define DGB200_LAYOUT_ROW_IDS 0 /* grouped_layout[m] = group of row m, -1 = padding */
 #define DGB200_LAYOUT_PSUM 1    /* grouped_layout[g] = end row of group g (use_psum_layout=True) */
+#define DGB200_LAYOUT_MASKED 2  /* dgb200_fp8_block_scaled_gemm: A and D are [num_groups, m, *], layout[g] = valid rows of group g */
+#define DGB200_LAYOUT_DENSE 3   /* dgb200_fp8_block_scaled_gemm: one group, no layout array */
 
 const char* dgb200_last_error(void);
 int dgb200_version(void);
@@ -461,6 +463,101 @@ int dgb200_nvfp4_mega_moe_bf16_input(void* y, const void* x, int64_t x_row_strid
 int dgb200_moe_dispatch_plan_noalloc(const int64_t* topk_idx, int32_t num_tokens, int32_t num_topk, int32_t num_experts,
                                      int32_t alignment, int32_t* dest_row, int32_t* expert_start, int32_t* expert_end,
                                      void* stream);
+
+/* FP8 GEMM whose operands carry an FP32 scale per block of 128 (any positive value, not only powers of two):
+ *   d[m, n] = c[m, n] + sum over K blocks kb of sfa[m, kb] * sfb[n / 128, kb] * sum_{k in kb} a[m, k] * b[n, k]
+ * The products of one K block are summed by the tensor core in FP32, the K blocks by FP32 multiply-adds with the (rounded) product of
+ * the two scales, in ascending order. The form the reference's GEMMs take with FP32 scales and disable_ue8m0_cast
+ * (csrc/apis/gemm.hpp:73-124, :166-297), which it builds for the previous architecture only.
+ *   a    e4m3 [m, k] (masked: [num_groups, m, k]), K-major, rows dense.
+ *   sfa  scale of row r and K block kb (of group g, masked only) at sfa[g * sfa_group_stride + r * sfa_row_stride + kb * sfa_k_stride].
+ *   b    e4m3 [num_groups, n, k], dense; b_mn_major != 0: [num_groups, k, n], dense (n a multiple of 16).
+ *   sfb  scale of the 128 x 128 block (nb, kb) of group g at sfb[g * sfb_group_stride + nb * sfb_n_stride + kb * sfb_k_stride].
+ *   d    bf16, or float with d_is_fp32, row stride d_row_stride elements; rows 16-byte aligned.
+ *   c    optional (dense form, float d): float [m, n], may be d itself with the same stride, must not overlap it otherwise.
+ *   layout, layout_kind, alignment, store_padding, expected_m (masked: steers tiling only): as in the GEMMs above. Rows outside
+ *        the groups are not written, save for padding rows with store_padding (psum) and the rest of a started 128-row tile (row
+ *        ids). Layout words that name rows past m, or groups that do not exist, are cut off there (row ids: reported in the status block).
+ * n % 8 == 0, k % 16 == 0 (last blocks may be short), at most 512 groups in the psum and masked layouts; a and b 16-byte aligned. */
+typedef struct dgb200_fp8_block_scaled_gemm_args {
+    size_t struct_size; /* sizeof(dgb200_fp8_block_scaled_gemm_args) */
+    const void* a;
+    const float* sfa;
+    const void* b;
+    const float* sfb;
+    void* d;
+    const float* c;
+    const int32_t* layout;
+    int64_t sfa_group_stride, sfa_row_stride, sfa_k_stride;
+    int64_t sfb_group_stride, sfb_n_stride, sfb_k_stride;
+    int64_t d_row_stride, c_row_stride;
+    int32_t m, n, k, num_groups;
+    int32_t layout_kind, alignment, store_padding, expected_m;
+    int32_t b_mn_major, d_is_fp32;
+} dgb200_fp8_block_scaled_gemm_args;
+int dgb200_fp8_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args* args, void* stream);
+
+/* BF16 rows -> E4M3 + one FP32 scale per gran_k (32 or 128) elements: sf = max(amax, 1e-4) / 448, q = e4m3(x / sf) (the quotient rounded to
+ * FP32, then to E4M3). Reference: per_token_cast_to_fp8(use_ue8m0=False), deep_gemm/utils/math.py:26-49. k % 16 == 0; sf row-major with
+ * sf_row_stride. A block that holds an infinity gets the scale infinity (its infinities become NaN, the rest 0); NaN stays NaN. */
+int dgb200_per_token_cast_to_fp8_f32_scales(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int32_t gran_k, void* q,
+                                            int64_t q_row_stride, float* sf, int64_t sf_row_stride, void* stream);
+
+/* BF16 [num_groups, rows, k] -> E4M3 + one FP32 scale per 128 x 128 block (edge blocks may be short), rounded as above; use_ue8m0 != 0: the
+ * scale is the smallest power of two not below it. Reference: per_block_cast_to_fp8, deep_gemm/utils/math.py:62-73. */
+int dgb200_per_block_cast_to_fp8(const void* x, int64_t x_group_stride, int64_t x_row_stride, int32_t num_groups, int32_t rows, int32_t k,
+                                 int32_t use_ue8m0, void* q, int64_t q_group_stride, int64_t q_row_stride, float* sf, int64_t sf_group_stride,
+                                 int64_t sf_row_stride, void* stream);
+
+/* Tokens sorted by expert and back, for callers that run the grouped GEMMs themselves (the layers do it inside their calls). No
+ * reference counterpart.
+ * Plan: a stable sort of the (token, k) entries by expert.
+ *   topk_idx  int64 [num_tokens, num_topk]; an index outside [0, num_experts) (-1 by convention) masks its entry.
+ *   dest_row  int32 [num_tokens, num_topk]: the entry's row in expert order, -1 = masked.
+ *   expert_start, expert_end  int32 [num_experts]: the segments; each starts at a multiple of `alignment`. expert_end is the psum
+ *             layout of the grouped GEMMs (of the same alignment).
+ *   workspace dgb200_moe_dispatch_plan_workspace_bytes(...) bytes of device memory (0: may be NULL); calls that may overlap need one each.
+ * num_topk <= 32, num_experts <= 1024. */
+int64_t dgb200_moe_dispatch_plan_workspace_bytes(int32_t num_tokens, int32_t num_topk, int32_t num_experts);
+int dgb200_moe_dispatch_plan(const int64_t* topk_idx, int32_t num_tokens, int32_t num_topk, int32_t num_experts, int32_t alignment,
+                             int32_t* dest_row, int32_t* expert_start, int32_t* expert_end, void* workspace, void* stream);
+
+/* rows[dest_row[t, k]] = x[t] for every entry that is not masked, byte for byte (x_row_bytes of any type), and likewise, with x_sf, the float
+ * scale rows. zero_padding != 0: the rows between each segment's end and its aligned end become zero (the K-grouped GEMMs ask for
+ * that). Rows behind the last segment are left as they are. capacity = rows of `rows`; num_tokens * num_topk + min(num_experts,
+ * num_tokens * num_topk) * (alignment - 1) always suffice; an entry whose row is not below it is left out and reported in the status block. */
+int dgb200_moe_permute(const void* x, int64_t x_row_bytes, int64_t x_row_stride_bytes, void* rows, int64_t rows_row_stride_bytes, const float* x_sf,
+                       int32_t sf_per_row, int64_t x_sf_row_stride, float* rows_sf, int64_t rows_sf_row_stride, const int32_t* dest_row,
+                       const int32_t* expert_end, int32_t num_tokens, int32_t num_topk, int32_t num_experts, int32_t alignment, int32_t capacity,
+                       int32_t zero_padding, void* stream);
+
+/* y[t] = sum over k of topk_weights[t, k] * rows[dest_row[t, k]], ascending k, FP32, one rounding; masked entries add nothing and neither their
+ * weight nor any row is read for them; topk_weights (float [num_tokens, num_topk]) NULL = 1, which makes it the gradient of
+ * dgb200_moe_permute. rows and y bf16, or float with is_fp32. */
+int dgb200_moe_unpermute(const void* rows, int64_t rows_row_stride, const float* topk_weights, const int32_t* dest_row, void* y, int64_t y_row_stride,
+                         int32_t num_tokens, int32_t num_topk, int32_t hidden, int32_t capacity, int32_t is_fp32, void* stream);
+
+/* Gradients of dgb200_moe_unpermute: d_rows[dest_row[t, k]] = topk_weights[t, k] * dy[t], the padding rows of every segment zero, the rows behind
+ * the last segment left as they are; d_weights (float [num_tokens, num_topk]) [t, k] = <rows[dest_row[t, k]], dy[t]> in FP32, 0 for masked
+ * entries. d_rows must not overlap rows or dy. */
+int dgb200_moe_unpermute_backward(const void* dy, int64_t dy_row_stride, const void* rows, int64_t rows_row_stride, const float* topk_weights,
+                                  const int32_t* dest_row, const int32_t* expert_end, void* d_rows, int64_t d_rows_row_stride, float* d_weights,
+                                  int32_t num_tokens, int32_t num_topk, int32_t num_experts, int32_t alignment, int32_t hidden, int32_t capacity,
+                                  int32_t is_fp32, void* stream);
+
+/* SwiGLU of rows [gate | up] (bf16 [rows, 2 * inter]): y = silu(min(gate, c)) * clamp(up, -c, c) with c = activation_clamp, <= 0 = no clamp;
+ * arithmetic in FP32, one rounding. With grouped_layout (psum layout of num_groups groups, NULL = all rows) only the rows
+ * below the last group's aligned end are computed, the others are left as they are. The cast form writes E4M3 and one FP32 scale per 128 columns
+ * (inter % 8 == 0), rounded as in dgb200_per_token_cast_to_fp8_f32_scales from the FP32 products. Backward: dx bf16
+ * [rows, 2 * inter] = [d_gate | d_up], zero where a clamp holds. Reference: the formula of its layer's epilogue
+ * (deep_gemm/include/deep_gemm/impls/sm100_fp8_fp4_mega_moe.cuh:1046-1126), a kernel of its own here. */
+int dgb200_swiglu(const void* x, int64_t x_row_stride, void* y, int64_t y_row_stride, int32_t rows, int32_t inter, const int32_t* grouped_layout,
+                  int32_t num_groups, int32_t alignment, float activation_clamp, void* stream);
+int dgb200_swiglu_per_token_cast_to_fp8(const void* x, int64_t x_row_stride, void* q, int64_t q_row_stride, float* sf, int64_t sf_row_stride,
+                                        int32_t rows, int32_t inter, const int32_t* grouped_layout, int32_t num_groups, int32_t alignment,
+                                        float activation_clamp, void* stream);
+int dgb200_swiglu_backward(const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride, void* dx, int64_t dx_row_stride, int32_t rows,
+                           int32_t inter, const int32_t* grouped_layout, int32_t num_groups, int32_t alignment, float activation_clamp, void* stream);
 
 /* Measurement hook: the NEXT dgb200_fp8_fp4_mega_moe call of this host thread records events[i] (cudaEvent_t
  * handles) on its stream at stage boundary i: 0 entry, 1 after the dispatch plan, 2 after the gather, 3 after L1,

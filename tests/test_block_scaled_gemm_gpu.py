@@ -1,0 +1,291 @@
+"""FP8 GEMMs with an FP32 scale per block of 128 (disable_ue8m0_cast=True) against the definition in FP64.
+
+Tolerance per element, derived and not fitted: products of E4M3 values are exact in FP32; every addition, in the tensor core (which may truncate) or
+in FP32, is off by at most 2^-23 of the largest partial sum, which S = sum |a| |b| |scales| bounds, k of them in the tensor core and one a K
+block outside, each there with a rounded product of scales (2 more); the result is rounded once to its type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def dg():
+    import deepgemm_b200
+    yield deepgemm_b200
+    from deepgemm_b200 import _lib
+    assert _lib.device_status()[0] == 0
+
+
+@pytest.fixture
+def tuning():
+    from deepgemm_b200 import _lib
+
+    def set_knob(name, value):
+        _lib.check(_lib.lib().dgb200_set_tuning(name.encode(), value))
+    yield set_knob
+    for name, value in (('block_n', 0), ('pair', -1)):
+        set_knob(name, value)
+
+
+def blocks(n):
+    return -(-n // 128)
+
+
+def operand(*shape, seed, block_rows):
+    """E4M3 values and positive scales that are no powers of two, over six orders of magnitude."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    q = (torch.randn(*shape, generator=g, device='cuda') * 40).clamp(-448, 448).to(torch.float8_e4m3fn)
+    rows = shape[-2] if block_rows == 1 else blocks(shape[-2])
+    sf = torch.exp(torch.randn(*shape[:-2], rows, blocks(shape[-1]), generator=g, device='cuda') * 2 - 4)
+    return q, sf
+
+
+def wide(q, sf, block_rows):
+    full = sf.double().repeat_interleave(128, dim=-1)[..., :q.shape[-1]]
+    if block_rows == 128:
+        full = full.repeat_interleave(128, dim=-2)[..., :q.shape[-2], :]
+    return q.double() * full
+
+
+def reference(a, b):
+    """(product, S) of a [m, k] and b [n, k] in FP64."""
+    aw, bw = wide(*a, 1), wide(*b, 128)
+    return aw @ bw.T, aw.abs() @ bw.abs().T
+
+
+def check(got, want, s, k, extra=0.0):
+    half_step = 2.0 ** -24 if got.dtype == torch.float32 else 2.0 ** -8
+    tol = s * (k + 3 * blocks(k) + 4) * 2.0 ** -23 + (want.abs() + extra) * half_step
+    over = (got.double() - want).abs() - tol * 1.01
+    assert torch.isfinite(got.float()).all()
+    assert (over <= 0).all(), f'{int((over > 0).sum())} values off, worst {float(over.max())}'
+
+
+SHAPES = [(1, 8, 16), (3, 24, 128), (7, 136, 272), (64, 64, 512), (128, 256, 1024), (129, 264, 144), (300, 520, 1040), (257, 2112, 896),
+          (1000, 1536, 640)]
+
+
+@pytest.mark.parametrize('m, n, k', SHAPES)
+@pytest.mark.parametrize('f32', [False, True])
+def test_dense(dg, m, n, k, f32):
+    a, b = operand(m, k, seed=1, block_rows=1), operand(n, k, seed=2, block_rows=128)
+    d = torch.full((m, n), float('nan'), dtype=torch.float32 if f32 else torch.bfloat16, device='cuda')
+    dg.fp8_gemm_nt(a, b, d, disable_ue8m0_cast=True)
+    check(d, *reference(a, b), k)
+
+
+@pytest.mark.parametrize('block_n, pair', [(128, 0), (256, 0), (256, 1)])
+@pytest.mark.parametrize('m, n, k', [(1, 8, 16), (128, 256, 1024), (129, 264, 144), (700, 1304, 2064)])
+@pytest.mark.parametrize('mn_major', [False, True])
+def test_dense_every_tile_form(dg, tuning, block_n, pair, m, n, k, mn_major):
+    if mn_major and n % 16 != 0:
+        n += 8
+    tuning('block_n', block_n)
+    tuning('pair', pair)
+    a, b = operand(m, k, seed=3, block_rows=1), operand(n, k, seed=4, block_rows=128)
+    used = (b[0].t().contiguous().t(), b[1]) if mn_major else b
+    want, s = reference(a, b)
+    for dtype in (torch.bfloat16, torch.float32):
+        d = torch.full((m, n), float('nan'), dtype=dtype, device='cuda')
+        dg.fp8_gemm_nt(a, used, d, disable_ue8m0_cast=True)
+        check(d, want, s, k)
+
+
+@pytest.mark.parametrize('where', ['apart', 'in place', 'strided', 'overlapping'])
+@pytest.mark.parametrize('m, n, k', [(5, 16, 144), (200, 392, 640)])
+def test_accumulator(dg, where, m, n, k):
+    a, b = operand(m, k, seed=5, block_rows=1), operand(n, k, seed=6, block_rows=128)
+    store = torch.randn(2 * m + 1, 2 * n, device='cuda')
+    d = store[:m, :n] if where != 'apart' else torch.empty(m, n, device='cuda')
+    c = {'apart': store[:m, :n].contiguous(), 'in place': d, 'strided': store[m:2 * m, n:], 'overlapping': store[1:m + 1, :n]}[where]
+    kept = c.clone()
+    want, s = reference(a, b)
+    dg.fp8_gemm_nt(a, b, d, c=c, disable_ue8m0_cast=True)
+    check(d, want + kept.double(), s, k, extra=kept.double().abs() + want.abs())
+
+
+def test_dense_nn_and_strided_scales_and_output(dg):
+    m, n, k = 150, 272, 528
+    a, b = operand(m, k, seed=7, block_rows=1), operand(n, k, seed=8, block_rows=128)
+    store = torch.full((m, n + 40), float('nan'), dtype=torch.bfloat16, device='cuda')
+    d = store[:, :n]
+    sfa = a[1].t().contiguous().t()  # MN-major scales
+    dg.fp8_gemm_nn((a[0], sfa), (b[0].t().contiguous(), b[1].t().contiguous()), d, disable_ue8m0_cast=True)
+    check(d, *reference(a, b), k)
+    assert torch.isnan(store[:, n:].float()).all()
+
+
+def grouped_case(ms, n, k, alignment, seed, tail=0):
+    starts, ends, at = [], [], 0
+    for x in ms:
+        starts.append(at)
+        ends.append(at + x)
+        at += -(-x // alignment) * alignment
+    rows = at + tail
+    a = operand(max(rows, 1), k, seed=seed, block_rows=1)
+    for s, e in zip(starts, ends):
+        a[0].view(torch.int8)[e:-(-e // alignment) * alignment] = 0
+    b = operand(len(ms), n, k, seed=seed + 1, block_rows=128)
+    return a, b, starts, ends, rows
+
+
+GROUPS = [[0], [1], [5, 0, 130], [128, 127, 129, 0, 1, 300], [0, 0, 600, 0]]
+
+
+@pytest.mark.parametrize('ms', GROUPS)
+@pytest.mark.parametrize('nn', [False, True])
+@pytest.mark.parametrize('alignment', [16, 128])
+@pytest.mark.parametrize('pair', [0, 1])
+def test_grouped_psum(dg, tuning, ms, nn, alignment, pair):
+    n, k = 400, 656
+    tuning('pair', pair)
+    if pair:
+        tuning('block_n', 256)
+    a, b, starts, ends, rows = grouped_case(ms, n, k, alignment, seed=11, tail=140)
+    layout = torch.tensor(ends, dtype=torch.int32, device='cuda')
+    d = torch.full((rows, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    gemm = dg.m_grouped_fp8_gemm_nn_contiguous if nn else dg.m_grouped_fp8_gemm_nt_contiguous
+    used = (b[0].transpose(1, 2).contiguous(), b[1].transpose(1, 2).contiguous()) if nn else b
+    dg.set_mk_alignment_for_contiguous_layout(alignment)
+    try:
+        for padding in (False, True):
+            d.fill_(float('nan'))
+            gemm(a, used, d, layout, disable_ue8m0_cast=True, use_psum_layout=True, ensure_zero_padding=padding)
+            written = torch.zeros(rows, dtype=torch.bool, device='cuda')
+            for g, (s, e) in enumerate(zip(starts, ends)):
+                if e > s:
+                    check(d[s:e], *reference((a[0][s:e], a[1][s:e]), (b[0][g], b[1][g])), k)
+                last = -(-e // alignment) * alignment if padding else e
+                assert (d[e:last] == 0).all()
+                written[s:last] = True
+            assert torch.isnan(d[~written].float()).all()
+    finally:
+        dg.set_mk_alignment_for_contiguous_layout(128)
+
+
+@pytest.mark.parametrize('ms', GROUPS[1:])
+def test_grouped_row_ids(dg, ms):
+    n, k = 264, 384
+    a, b, starts, ends, rows = grouped_case(ms, n, k, 128, seed=13, tail=256)
+    ids = torch.full((rows,), -1, dtype=torch.int32)
+    for g, (s, e) in enumerate(zip(starts, ends)):
+        ids[s:e] = g
+    d = torch.full((rows, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    dg.m_grouped_fp8_gemm_nt_contiguous(a, b, d, ids.cuda(), disable_ue8m0_cast=True)
+    for g, (s, e) in enumerate(zip(starts, ends)):
+        if e > s:
+            check(d[s:e], *reference((a[0][s:e], a[1][s:e]), (b[0][g], b[1][g])), k)
+    assert torch.isnan(d[-(-max(ends) // 128) * 128:].float()).all()
+
+
+@pytest.mark.parametrize('max_m, counts', [(4, [0, 1, 4]), (96, [96, 0, 33]), (200, [200, 129, 128, 1]), (300, [0, 300])])
+@pytest.mark.parametrize('pair', [-1, 1])
+def test_masked(dg, tuning, max_m, counts, pair):
+    n, k, g = 520, 400, len(counts)
+    if pair == 1:
+        tuning('block_n', 256)
+        tuning('pair', 1)
+    a, b = operand(g, max_m, k, seed=17, block_rows=1), operand(g, n, k, seed=18, block_rows=128)
+    d = torch.full((g, max_m, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    dg.m_grouped_fp8_gemm_nt_masked(a, b, d, torch.tensor(counts, dtype=torch.int32, device='cuda'), max(1, max_m // 2), disable_ue8m0_cast=True)
+    for i, m in enumerate(counts):
+        if m:
+            check(d[i, :m], *reference((a[0][i, :m], a[1][i, :m]), (b[0][i], b[1][i])), k)
+        assert torch.isnan(d[i, m:].float()).all()
+
+
+def test_values_that_a_tile_holds_but_a_group_does_not(dg):
+    """NaN in rows of A behind a group, in the scales of rows that are not stored and in the weights of the next group, whose rows follow
+    the short last K block in memory: none of it reaches a result."""
+    n, k, ms = 136, 144, [3, 70]
+    for nn in (False, True):
+        a, b, starts, ends, rows = grouped_case(ms, n if not nn else 144, k, 128, seed=19)
+        n_used = b[0].shape[1]
+        codes = a[0].view(torch.uint8)
+        codes[ends[1]:] = 0x7f
+        codes[ends[0]:128] = 0x7f
+        a[1][ends[0]:128] = float('nan')
+        want = [reference((a[0][s:e], a[1][s:e]), (b[0][g], b[1][g])) for g, (s, e) in enumerate(zip(starts, ends))]
+        for bad in (0, 1):
+            q = b[0].clone()
+            q.view(torch.uint8)[bad] = 0x7f
+            used = (q.transpose(1, 2).contiguous(), b[1].transpose(1, 2).contiguous()) if nn else (q, b[1])
+            d = torch.zeros((rows, n_used), dtype=torch.bfloat16, device='cuda')
+            gemm = dg.m_grouped_fp8_gemm_nn_contiguous if nn else dg.m_grouped_fp8_gemm_nt_contiguous
+            gemm(a, used, d, torch.tensor(ends, dtype=torch.int32, device='cuda'), disable_ue8m0_cast=True, use_psum_layout=True,
+                 ensure_zero_padding=False)
+            other = 1 - bad
+            check(d[starts[other]:ends[other]], *want[other], k)
+            assert torch.isnan(d[starts[bad]:ends[bad]].float()).all()
+
+
+def test_layout_words_past_the_buffer_are_cut_off(dg):
+    n, k, rows = 128, 128, 256
+    store = torch.full((rows + 512, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    a, b = operand(rows, k, seed=23, block_rows=1), operand(3, n, k, seed=24, block_rows=128)
+    for words in ([-5, 300, 2 ** 31 - 1], [256, 100, 10 ** 6]):
+        dg.m_grouped_fp8_gemm_nt_contiguous(a, b, store[:rows], torch.tensor(words, dtype=torch.int32, device='cuda'), disable_ue8m0_cast=True,
+                                            use_psum_layout=True)
+        assert torch.isnan(store[rows:].float()).all()
+    am, d = operand(3, 64, k, seed=25, block_rows=1), torch.full((4, 64, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    dg.m_grouped_fp8_gemm_nt_masked(am, b, d[:3], torch.tensor([-3, 1000, 64], dtype=torch.int32, device='cuda'), 64, disable_ue8m0_cast=True)
+    assert torch.isnan(d[0].float()).all() and torch.isnan(d[3].float()).all() and torch.isfinite(d[1:3].float()).all()
+
+
+def test_row_ids_of_no_group_are_reported(dg):
+    from deepgemm_b200 import _lib
+    n, k = 128, 128
+    a, b = operand(256, k, seed=27, block_rows=1), operand(2, n, k, seed=28, block_rows=128)
+    ids = torch.tensor([0] * 128 + [7] * 128, dtype=torch.int32, device='cuda')
+    d = torch.full((256, n), float('nan'), dtype=torch.bfloat16, device='cuda')
+    dg.m_grouped_fp8_gemm_nt_contiguous(a, b, d, ids, disable_ue8m0_cast=True)
+    with pytest.raises(RuntimeError, match='code 6'):
+        _lib.device_status()
+    check(d[:128], *reference((a[0][:128], a[1][:128]), (b[0][0], b[1][0])), k)
+    assert torch.isnan(d[128:].float()).all()
+
+
+def test_same_bits_in_a_graph_on_side_streams_and_in_every_run(dg):
+    m, n, k = 260, 384, 768
+    cases = [(operand(m, k, seed=31 + i, block_rows=1), operand(n, k, seed=41 + i, block_rows=128)) for i in range(2)]
+    want = []
+    for a, b in cases:
+        d = torch.empty((m, n), dtype=torch.bfloat16, device='cuda')
+        dg.fp8_gemm_nt(a, b, d, disable_ue8m0_cast=True)
+        want.append(d)
+    outs = [torch.empty_like(w) for w in want]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (a, b), out, stream in zip(cases, outs, streams):
+            with torch.cuda.stream(stream):
+                dg.fp8_gemm_nt(a, b, out, disable_ue8m0_cast=True)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    graph, static = torch.cuda.CUDAGraph(), [t.clone() for t in (*cases[0][0], *cases[0][1])]
+    out = torch.empty_like(want[0])
+    with torch.cuda.graph(graph):
+        dg.fp8_gemm_nt((static[0], static[1]), (static[2], static[3]), out, disable_ue8m0_cast=True)
+    for i in (1, 0):
+        for t, new in zip(static, (*cases[i][0], *cases[i][1])):
+            t.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+
+
+def test_limited_sms_give_the_same_bits(dg):
+    m, n, k = 600, 1024, 512
+    a, b = operand(m, k, seed=51, block_rows=1), operand(n, k, seed=52, block_rows=128)
+    outs = []
+    for sms in (0, 1, 7):
+        dg.set_num_sms(sms)
+        try:
+            d = torch.empty((m, n), dtype=torch.bfloat16, device='cuda')
+            dg.fp8_gemm_nt(a, b, d, disable_ue8m0_cast=True)
+        finally:
+            dg.set_num_sms(0)
+        outs.append(d)
+    check(outs[0], *reference(a, b), k)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
