@@ -30,6 +30,7 @@ struct BlockScaledParams {
     int mode;  // kModeDense / kModeRowIds / kModePsum / kModeMasked (A and D [G, m, *])
     int m, n, k, num_groups, alignment, store_padding;
     int b_mn_major;   // B is [groups, k, n] with n contiguous
+    int sf_vec;       // the scales of four consecutive K blocks lie in 16 aligned bytes, for a as for b
     int a_box_rows;   // rows of A that one load brings: 128, or fewer where no tile has more
 };
 
@@ -38,23 +39,53 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3_f32(uint32_t m, uint32_t 
     return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-__device__ __forceinline__ void tcgen05_mma_f8f6f4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-        "}\n"
-        :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+// Shared-memory descriptors of 128-byte-swizzled tiles whose 8-row groups are 1024 bytes apart, as two words: the upper one is the same
+// for every tile, the lower one holds the address (and, MN-major, the 16 KB between 128-byte chunks along N).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, bool mn_major) {
+    return ((smem_addr & 0x3ffffu) >> 4) | (mn_major ? (16384u >> 4) << 16 : 0u);
 }
-__device__ __forceinline__ void tcgen05_mma_f8f6f4_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-        "}\n"
-        :: "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+
+// D[tmem] = A B^T of one K block: four MMAs of K = 32, the first one overwrites D. kPair: on both CTAs of the pair.
+template <bool kPair>
+__device__ __forceinline__ void mma_k_block(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t b_step, uint32_t idesc) {
+#pragma unroll
+    for (uint32_t k4 = 0; k4 < 4; ++k4) {
+        if constexpr (kPair)
+            asm volatile(
+                "{\n\t"
+                ".reg .pred p;\n\t"
+                ".reg .b64 a, b;\n\t"
+                "mov.b64 a, {%1, %4};\n\t"
+                "mov.b64 b, {%2, %4};\n\t"
+                "setp.ne.b32 p, %5, 0;\n\t"
+                "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n\t"
+                "}\n"
+                :: "r"(tmem_d), "r"(a_lo + k4 * 2), "r"(b_lo + k4 * b_step), "r"(idesc), "n"(kDescHi), "r"(k4) : "memory");
+        else
+            asm volatile(
+                "{\n\t"
+                ".reg .pred p;\n\t"
+                ".reg .b64 a, b;\n\t"
+                "mov.b64 a, {%1, %4};\n\t"
+                "mov.b64 b, {%2, %4};\n\t"
+                "setp.ne.b32 p, %5, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t"
+                "}\n"
+                :: "r"(tmem_d), "r"(a_lo + k4 * 2), "r"(b_lo + k4 * b_step), "r"(idesc), "n"(kDescHi), "r"(k4) : "memory");
+    }
+}
+
+// Two FP32 multiply-adds in one instruction: each result is what fmaf gives.
+__device__ __forceinline__ void fma_f32x2(float& a0, float& a1, uint32_t x0, uint32_t x1, float s) {
+    asm volatile("{\n\t"
+        ".reg .b64 x, s, a;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 s, {%4, %4};\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "fma.rn.f32x2 a, x, s, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t"
+        "}\n" : "+f"(a0), "+f"(a1) : "r"(x0), "r"(x1), "f"(s));
 }
 
 // Tiled 3-D loads (same rules as the 2-D ones): into this CTA's shared memory, completing on its own barrier or on one of the pair's.
@@ -70,16 +101,38 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
         :: "r"(smem_u32(smem_dst)), "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+constexpr int kScaleKb = 4;  // K blocks whose scales are loaded together
+
+// Scales of up to kScaleKb K blocks (`left` of them exist, 0 for the others): one 16-byte load where that is allowed. Lanes hold rows
+// far apart, so that every load instruction costs 32 cache lookups whatever its width.
+__device__ __forceinline__ void load_scales(const float* from, long long k_stride, int left, bool whole, float* to) {
+    if (whole && left >= kScaleKb) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(from));
+        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleKb; ++i) to[i] = i < left ? __ldg(from + i * k_stride) : 0.0f;
+}
+
 template <int BLOCK_N, int kStages, bool kPair>
 struct BlockScaledSmem {
+    static constexpr int kSumWarps = 8;
+    static constexpr int kAccums = BLOCK_N == 256 ? 2 : 4;  // accumulators in tensor memory: K blocks between the MMAs and the sums
+    // A slot of scales is written for K block i when the MMAs of K block i - kAccums are complete, which had waited until every summing
+    // warp had left K block i - 2 kAccums, the slot's last user.
+    static constexpr int kScaleSlots = 2 * kAccums;
+    static constexpr int kScaleSlotBytes = 2 * 128 * 4;  // [half of the tile's columns][row]
+    static constexpr int kSlabBytes = 64;                // epilogue staging: bytes of each of a warp's 32 rows
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = BLOCK_N * 128 / (kPair ? 2 : 1);
     static constexpr int kOffA = 0;
     static constexpr int kOffB = kOffA + kStages * kABytes;
-    static constexpr int kOffStage = kOffB + kStages * kBBytes;  // epilogue: 32 rows x 64 bytes per warp
-    static constexpr int kOffBar = kOffStage + 8 * 2048;
-    static constexpr int kNumBars = 2 * kStages + 2 * (512 / (BLOCK_N < 64 ? 64 : BLOCK_N));
-    static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+    static constexpr int kOffStage = kOffB + kStages * kBBytes;
+    static constexpr int kOffScales = kOffStage + kSumWarps * 32 * kSlabBytes;
+    static constexpr int kOffBar = kOffScales + kScaleSlots * kScaleSlotBytes;
+    static constexpr int kNumBars = 2 * kStages + kAccums;
+    static constexpr int kOffMisc = kOffBar + (kNumBars * 8 + 15) / 16 * 16;
     static constexpr int kOffGroups = kOffMisc + 16;
     static constexpr int kTotal = kOffGroups + 3 * kMaxCachedGroups * 4;
     static constexpr int kDynamicBytes = kTotal + 1024;  // slack to align the base to 1024 B
@@ -152,7 +205,7 @@ struct BlockScaledScheduler {
     }
 };
 
-constexpr int kRegsBsControl = 56, kRegsBsSum = 224;  // 128 x 56 + 256 x 224 = 384 x 168, what the block is launched with
+constexpr int kRegsBsControl = 72, kRegsBsSum = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
 
 template <int BLOCK_N, int kStages, bool kF32, bool kPair>
 __global__ void __launch_bounds__(kGemmThreads, 1)
@@ -161,8 +214,11 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     using L = BlockScaledSmem<BLOCK_N, kStages, kPair>;
     using Sched = BlockScaledScheduler<BLOCK_N, kPair>;
     constexpr int kCtas = kPair ? 2 : 1;
-    constexpr int kAccums = 512 / (BLOCK_N < 64 ? 64 : BLOCK_N);  // accumulators in tensor memory: K blocks in flight
-    constexpr int kCols = BLOCK_N / 2;                            // columns a thread sums
+    constexpr int kAccums = L::kAccums;
+    constexpr uint32_t kAccumCols = BLOCK_N < 64 ? 64 : BLOCK_N;
+    constexpr int kSumWarps = L::kSumWarps;
+    constexpr int kThreads = kGemmThreads;
+    constexpr int kCols = BLOCK_N / (kSumWarps / 4);  // columns a thread sums
     static_assert(BLOCK_N == 32 || BLOCK_N == 64 || BLOCK_N == 128 || BLOCK_N == 256, "tile width");
     static_assert(!kPair || BLOCK_N == 256, "pairs work on 256 x 256 tiles");
     static_assert(L::kDynamicBytes <= 232448, "shared memory budget");
@@ -172,7 +228,6 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
     uint64_t* empty_bar = full_bar + kStages;
     uint64_t* tmem_full_bar = empty_bar + kStages;
-    uint64_t* tmem_empty_bar = tmem_full_bar + kAccums;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kOffMisc + 4);
     int* table = reinterpret_cast<int*>(smem + L::kOffGroups);
@@ -184,12 +239,13 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(full_bar + i, 2 * kCtas);  // the A loader and the B loader of every CTA
-            mbar_init(empty_bar + i, 1);         // tcgen05.commit of the MMA issuer
+            // K block i may be multiplied when its operands are there (the A loader and the B loader of every CTA) and its accumulator has been
+            // read (lane 0 of every summing warp, when it has taken K block i - kAccums): one barrier, one wait of the MMA issuer.
+            mbar_init(full_bar + i, (2 + kSumWarps) * kCtas);
+            mbar_init(empty_bar + i, 1);  // a summing warp of this CTA that has seen the K block's MMAs complete
         }
         for (int i = 0; i < kAccums; ++i) {
-            mbar_init(tmem_full_bar + i, 1);
-            mbar_init(tmem_empty_bar + i, 8 * kCtas);  // lane 0 of each summing warp
+            mbar_init(tmem_full_bar + i, 2);  // tcgen05.commit of the MMA issuer, and this CTA's scale warp: products and scales are there
         }
         fence_mbar_init();
         prefetch_tensormap(&tm_a);
@@ -198,7 +254,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     pdl_prologue();  // everything above touches only this CTA's shared memory and the kernel's own parameters
     if (p.mode == kModePsum || p.mode == kModeMasked) {
         int* tiles_end = table + 2 * kMaxCachedGroups;
-        for (int i = threadIdx.x; i < p.num_groups; i += kGemmThreads) {
+        for (int i = threadIdx.x; i < p.num_groups; i += kThreads) {
             int first, count;
             Sched::group_extent(p, i, first, count);
             table[i] = first;
@@ -288,151 +344,180 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             }
         } else if (warp == 1 && leader_cta) {
             // ------------------------------------------------------------ MMA issuer: one accumulator per K block
+            // The summing warps leave this one few issue slots, and a K block is only 512 cycles (256 for a 128-wide tile) of MMAs: its loop holds
+            // as few instructions as possible. Descriptors are one word each, moved on by additions; there is one barrier to
+            // wait for and one commit.
             const bool elected = elect_one();
             Sched sched(p, table);
             BlockScaledTile t;
-            uint32_t stage = 0, phase = 0, as = 0, aphase = 0;
             const bool b_mn = BLOCK_N >= 128 && p.b_mn_major;
             const uint32_t idesc = make_idesc_e4m3_f32(128 * kCtas, BLOCK_N) | (b_mn ? (1u << 16) : 0u);
-            const uint32_t a_base = smem_u32(smem + L::kOffA), b_base = smem_u32(smem + L::kOffB);
+            const uint32_t a_first = desc_lo(smem_u32(smem + L::kOffA), false), b_first = desc_lo(smem_u32(smem + L::kOffB), b_mn);
             const uint32_t b_step = b_mn ? 256u : 2u;  // 32 K rows of 128 bytes, or 32 bytes inside the swizzle span
+            uint32_t stage = 0, phase = 0, as = 0;
+            uint32_t a_lo = a_first, b_lo = b_first;
             bool ok = true;
             while (ok && sched.next(t)) {
                 if (t.group < 0) continue;
+#pragma unroll 1
                 for (int kb = 0; kb < num_kb; ++kb) {
-                    ok = mbar_wait(tmem_empty_bar + as, aphase ^ 1, abort_flag, kTimeoutTmemEmpty, kb) &&
-                         mbar_wait(full_bar + stage, phase, abort_flag, kTimeoutFull, kb);
+                    ok = mbar_wait(full_bar + stage, phase, abort_flag, kTimeoutFull, kb);
                     if (!ok) break;
                     tcgen05_fence_after();
                     if (elected) {
-                        const uint64_t adesc = make_kmajor_sw128_desc(a_base + stage * L::kABytes);
-                        const uint64_t bdesc = b_mn ? make_mnmajor_sw128_desc(b_base + stage * L::kBBytes, 16384)
-                                                    : make_kmajor_sw128_desc(b_base + stage * L::kBBytes);
-                        const uint32_t acc = tmem_base + as * (BLOCK_N < 64 ? 64 : BLOCK_N);
-#pragma unroll
-                        for (uint32_t k4 = 0; k4 < 4; ++k4) {
-                            if constexpr (kPair) tcgen05_mma_f8f6f4_pair(acc, adesc + k4 * 2, bdesc + k4 * b_step, idesc, k4);
-                            else tcgen05_mma_f8f6f4(acc, adesc + k4 * 2, bdesc + k4 * b_step, idesc, k4);
-                        }
-                        if constexpr (kPair) {
-                            tcgen05_commit_pair(empty_bar + stage, 3);
-                            tcgen05_commit_pair(tmem_full_bar + as, 3);
-                        } else {
-                            tcgen05_commit(empty_bar + stage);
-                            tcgen05_commit(tmem_full_bar + as);
-                        }
+                        mma_k_block<kPair>(tmem_base + as * kAccumCols, a_lo, b_lo, b_step, idesc);
+                        if constexpr (kPair) tcgen05_commit_pair(tmem_full_bar + as, 3);
+                        else tcgen05_commit(tmem_full_bar + as);
                     }
                     __syncwarp();
-                    if (++stage == kStages) { stage = 0; phase ^= 1; }
-                    if (++as == kAccums) { as = 0; aphase ^= 1; }
+                    as = as + 1 == kAccums ? 0 : as + 1;
+                    a_lo += L::kABytes >> 4;
+                    b_lo += L::kBBytes >> 4;
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                        a_lo = a_first;
+                        b_lo = b_first;
+                    }
+                }
+            }
+        } else if (warp == 2) {
+            // ------------------------------------------------------------ scales: sfa[row] * sfb[column block]
+            // The loads of four K blocks are under way together, well ahead of their use; read by the summing warps
+            // themselves, one K block ahead, their latency was a fifth of the kernel.
+            Sched sched(p, table);
+            BlockScaledTile t;
+            uint32_t as = 0, phase = 0, slot = 0;
+            bool ok = true;
+            while (ok && sched.next(t)) {
+                if (t.group < 0) continue;
+                const long long group = t.group;
+                const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + static_cast<long long>(t.row0 + static_cast<int>(lane)) * p.sfa_row_stride;
+                const float* sfb[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    sfb[h] = p.sfb + group * p.sfb_group_stride + static_cast<long long>(min(t.n0 + h * (BLOCK_N / 2), p.n - 1) / 128) * p.sfb_n_stride;
+                for (int kb = 0; ok && kb < num_kb; kb += kScaleKb) {
+                    float a[4][kScaleKb], b[2][kScaleKb];
+                    const bool whole = p.sf_vec && kb + kScaleKb <= num_kb;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)  // rows that are not stored need no scale: none is read for them
+                        load_scales(sfa + 32 * j * p.sfa_row_stride + kb * p.sfa_k_stride, p.sfa_k_stride,
+                                    static_cast<int>(lane) + 32 * j < t.rows ? num_kb - kb : 0, whole, a[j]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) load_scales(sfb[h] + kb * p.sfb_k_stride, p.sfb_k_stride, num_kb - kb, whole, b[h]);
+#pragma unroll
+                    for (int i = 0; i < kScaleKb; ++i) {
+                        if (!ok || kb + i >= num_kb) break;
+                        ok = mbar_wait(tmem_full_bar + as, phase ^ 1, abort_flag, kTimeoutTmemFull, kb);  // K block kb + i - kAccums
+                        if (!ok) break;
+                        float* to = reinterpret_cast<float*>(smem + L::kOffScales + slot * L::kScaleSlotBytes) + lane;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) to[h * 128 + 32 * j] = a[j][i] * b[h][i];
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(tmem_full_bar + as);
+                        if (++as == kAccums) { as = 0; phase ^= 1; }
+                        if (++slot == L::kScaleSlots) slot = 0;
+                    }
                 }
             }
         }
     } else {
         setmaxnreg_inc<kRegsBsSum>();
-        // ---------------------------------------------------------------- running sums and epilogue (8 warps)
-        const uint32_t q = warp & 3, half = (warp - 4) >> 2;
+        // ---------------------------------------------------------------- running sums and epilogue
+        const uint32_t q = warp & 3, half = (warp - 4) >> 2;  // lane quarter of tensor memory, half of the tile's columns
         const int r = static_cast<int>(q * 32 + lane);
-        uint8_t* stage_buf = smem + L::kOffStage + (warp - 4) * 2048;
+        uint8_t* stage_buf = smem + L::kOffStage + (warp - 4) * (32 * L::kSlabBytes);
+        // the barriers of the MMA issuer's CTA
+        const uint32_t issuer_full = kPair ? map_to_cta(smem_u32(full_bar), 0) : smem_u32(full_bar);
+        auto give_accumulator = [&](uint32_t to_stage) {
+            if constexpr (kPair) mbar_arrive_cluster(issuer_full + to_stage * 8);
+            else mbar_arrive(full_bar + to_stage);
+        };
+        static_assert(kAccums <= kStages, "a K block's barrier is past its previous use when its accumulator is given back");
+        if (lane == 0) {
+            for (int i = 0; i < kAccums; ++i) give_accumulator(i);  // all are free
+        }
+        const uint32_t tmem_half = tmem_base + ((q * 32u) << 16) + half * kCols;
+        const float* const my_scales = reinterpret_cast<const float*>(smem + L::kOffScales) + half * 128 + r;
         Sched sched(p, table);
         BlockScaledTile t;
-        uint32_t as = 0, aphase = 0;
+        // stage of the K block at hand and of the one that will use its accumulator next (kAccums K blocks later)
+        uint32_t as = 0, aphase = 0, stage = 0, next_stage = kAccums % kStages, slot = 0;
         bool ok = true;
         while (ok && sched.next(t)) {
             if (t.group < 0) continue;
             const bool warp_has_rows = static_cast<int>(q * 32) < t.rows;
-            const int col0 = t.n0 + static_cast<int>(half) * kCols;
-            const long long group = t.group;
-            // rows that are not stored take the scale of the last one that is: never an address outside the tensor
-            const long long sf_row = t.row0 + min(r, max(t.rows - 1, 0));
-            const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + sf_row * p.sfa_row_stride;
-            const float* sfb = p.sfb + group * p.sfb_group_stride + static_cast<long long>(min(col0, p.n - 1) / 128) * p.sfb_n_stride;
             float acc[kCols];
 #pragma unroll
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
-            // scales two K blocks ahead of their use
-            float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
-            if (warp_has_rows) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (i < num_kb) {
-                        sa[i] = __ldg(sfa + i * p.sfa_k_stride);
-                        sb[i] = __ldg(sfb + i * p.sfb_k_stride);
-                    }
-            }
+#pragma unroll 1
             for (int kb = 0; kb < num_kb; ++kb) {
-                const float s = sa[0] * sb[0];
-                sa[0] = sa[1];
-                sb[0] = sb[1];
-                if (warp_has_rows && kb + 2 < num_kb) {
-                    sa[1] = __ldg(sfa + (kb + 2) * p.sfa_k_stride);
-                    sb[1] = __ldg(sfb + (kb + 2) * p.sfb_k_stride);
-                }
                 ok = mbar_wait(tmem_full_bar + as, aphase, abort_flag, kTimeoutTmemFull, kb);
                 if (!ok) break;
                 tcgen05_fence_after();
                 if (warp_has_rows) {
-                    const uint32_t tmem_row = tmem_base + as * (BLOCK_N < 64 ? 64 : BLOCK_N) + ((q * 32u) << 16) + half * kCols;
-                    if constexpr (kCols >= 64) {
-                        uint32_t v[2][32];
-                        tmem_ld_32x32b_x32(tmem_row, v[0]);
+                    constexpr int kChunk = 16;  // columns per load; the next load is under way while a chunk is added
+                    const uint32_t tmem_row = tmem_half + as * kAccumCols;
+                    uint32_t v[2][kChunk];
+                    tmem_ld_32x32b_x16(tmem_row, v[0]);
+                    const float s = my_scales[slot * (L::kScaleSlotBytes / 4)];
 #pragma unroll
-                        for (int c = 0; c < kCols / 32; ++c) {
-                            tmem_ld_wait();
-                            if (c + 1 < kCols / 32) tmem_ld_32x32b_x32(tmem_row + (c + 1) * 32, v[(c + 1) & 1]);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), s, acc[c * 32 + i]);
-                        }
-                    } else {
-                        uint32_t v[kCols];
-#pragma unroll
-                        for (int c = 0; c < kCols / 16; ++c) tmem_ld_32x32b_x16(tmem_row + c * 16, v + c * 16);
+                    for (int c = 0; c < kCols / kChunk; ++c) {
                         tmem_ld_wait();
+                        if (c + 1 < kCols / kChunk) tmem_ld_32x32b_x16(tmem_row + (c + 1) * kChunk, v[(c + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < kCols; ++i) acc[i] = fmaf(__uint_as_float(v[i]), s, acc[i]);
+                        for (int i = 0; i < kChunk; i += 2) fma_f32x2(acc[c * kChunk + i], acc[c * kChunk + i + 1], v[c & 1][i], v[c & 1][i + 1], s);
                     }
                 }
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (leader_cta) mbar_arrive(tmem_empty_bar + as);
-                    else mbar_arrive_cluster(map_to_cta(smem_u32(tmem_empty_bar + as), 0));
+                    give_accumulator(next_stage);                  // this warp has read the accumulator (and the scales)
+                    if (warp == 4) mbar_arrive(empty_bar + stage);  // the K block's operands have been read
                 }
                 if (++as == kAccums) { as = 0; aphase ^= 1; }
+                if (++stage == kStages) stage = 0;
+                if (++next_stage == kStages) next_stage = 0;
+                if (++slot == L::kScaleSlots) slot = 0;
             }
             if (!ok) break;
             if (!warp_has_rows) continue;
-            // Store: a slab of 32 rows x 64 bytes at a time is turned through shared memory (16-byte chunks, XOR-swizzled), so that a
-            // store instruction of the warp writes eight rows' 64 contiguous bytes instead of 16 bytes of 32 rows.
-            constexpr int kSlab = kF32 ? 16 : 32;  // columns
+            const int col0 = t.n0 + static_cast<int>(half) * kCols;
+            // Store: a slab of 32 rows x 64 (or 32) bytes at a time is turned through shared memory (16-byte chunks, XOR-swizzled), so
+            // that a store instruction of the warp writes whole sectors of eight (sixteen) rows instead of 16 bytes of 32 rows.
+            constexpr int kChunks = L::kSlabBytes / 16;             // of a row of the slab
+            constexpr int kPerChunk = kF32 ? 4 : 8;                 // columns
+            constexpr int kSlab = kChunks * kPerChunk;
             constexpr int kSlabs = (kCols + kSlab - 1) / kSlab;
-            const long long row_base = (p.mode == kModeMasked ? group * p.m : 0) + t.row0 + static_cast<int>(q * 32);
+            auto place = [&](int row, int chunk) {
+                return reinterpret_cast<uint4*>(stage_buf + row * L::kSlabBytes + ((chunk ^ ((row * L::kSlabBytes / 128) & (kChunks - 1))) << 4));
+            };
+            const long long row_base = (p.mode == kModeMasked ? static_cast<long long>(t.group) * p.m : 0) + t.row0 + static_cast<int>(q * 32);
             const int rows_here = t.rows - static_cast<int>(q * 32);
 #pragma unroll
             for (int s = 0; s < kSlabs; ++s) {
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 o;
-                    if constexpr (kF32) {
-                        const float* a = acc + s * kSlab + i * 4;
-                        o = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
-                    } else if (s * kSlab + i * 8 < kCols) {
-                        const float* a = acc + s * kSlab + i * 8;
-                        o = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
-                    } else {
-                        o = make_uint4(0, 0, 0, 0);
-                    }
-                    *reinterpret_cast<uint4*>(stage_buf + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = o;
+                for (int i = 0; i < kChunks; ++i) {
+                    const int at = s * kSlab + i * kPerChunk;
+                    if (at >= kCols) continue;
+                    const float* a = acc + at;
+                    if constexpr (kF32)
+                        *place(lane, i) = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+                    else
+                        *place(lane, i) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
                 }
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = static_cast<int>(lane >> 2) + 8 * j, chunk = static_cast<int>(lane & 3);
-                    const int in_half = s * kSlab + chunk * (kF32 ? 4 : 8);
-                    const int col = col0 + in_half;
-                    if (row >= rows_here || in_half >= kCols || col >= p.n) continue;  // n is a multiple of 8: a chunk is inside or outside
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage_buf + row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
+                for (int j = 0; j < kChunks; ++j) {
+                    const int row = static_cast<int>(lane) / kChunks + 32 / kChunks * j, chunk = static_cast<int>(lane) % kChunks;
+                    const int in_part = s * kSlab + chunk * kPerChunk;
+                    const int col = col0 + in_part;
+                    if (row >= rows_here || in_part >= kCols || col >= p.n) continue;  // n is a multiple of 8: a chunk is inside or outside
+                    const uint4 v = *place(row, chunk);
                     const long long at = (row_base + row) * p.d_row_stride + col;
                     if constexpr (kF32) {
                         float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));

@@ -93,6 +93,8 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     p.alignment = dense || masked ? 128 : a.alignment;
     p.store_padding = a.store_padding;
     p.b_mn_major = a.b_mn_major ? 1 : 0;
+    p.sf_vec = a.sfa_k_stride == 1 && a.sfb_k_stride == 1 && aligned_to(a.sfa, 16) && aligned_to(a.sfb, 16) && a.sfa_row_stride % 4 == 0 &&
+               a.sfb_n_stride % 4 == 0 && a.sfa_group_stride % 4 == 0 && a.sfb_group_stride % 4 == 0;
     int sms = 0;
     if (const int rc = effective_num_sms(&sms)) return rc;
 
