@@ -242,7 +242,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             // K block i may be multiplied when its operands are there (the A loader and the B loader of every CTA) and its accumulator has been
             // read (lane 0 of every summing warp, when it has taken K block i - kAccums): one barrier, one wait of the MMA issuer.
             mbar_init(full_bar + i, (2 + kSumWarps) * kCtas);
-            mbar_init(empty_bar + i, 1);  // a summing warp of this CTA that has seen the K block's MMAs complete
+            mbar_init(empty_bar + i, 1);  // tcgen05.commit of the MMA issuer
         }
         for (int i = 0; i < kAccums; ++i) {
             mbar_init(tmem_full_bar + i, 2);  // tcgen05.commit of the MMA issuer, and this CTA's scale warp: products and scales are there
@@ -345,8 +345,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
         } else if (warp == 1 && leader_cta) {
             // ------------------------------------------------------------ MMA issuer: one accumulator per K block
             // The summing warps leave this one few issue slots, and a K block is only 512 cycles (256 for a 128-wide tile) of MMAs: its loop holds
-            // as few instructions as possible. Descriptors are one word each, moved on by additions; there is one barrier to
-            // wait for and one commit.
+            // few instructions. Descriptors are one word each, moved on by additions, and there is one barrier to wait for.
             const bool elected = elect_one();
             Sched sched(p, table);
             BlockScaledTile t;
@@ -366,8 +365,13 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                     tcgen05_fence_after();
                     if (elected) {
                         mma_k_block<kPair>(tmem_base + as * kAccumCols, a_lo, b_lo, b_step, idesc);
-                        if constexpr (kPair) tcgen05_commit_pair(tmem_full_bar + as, 3);
-                        else tcgen05_commit(tmem_full_bar + as);
+                        if constexpr (kPair) {
+                            tcgen05_commit_pair(tmem_full_bar + as, 3);
+                            tcgen05_commit_pair(empty_bar + stage, 3);
+                        } else {
+                            tcgen05_commit(tmem_full_bar + as);
+                            tcgen05_commit(empty_bar + stage);
+                        }
                     }
                     __syncwarp();
                     as = as + 1 == kAccums ? 0 : as + 1;
@@ -393,19 +397,18 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                 if (t.group < 0) continue;
                 const long long group = t.group;
                 const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + static_cast<long long>(t.row0 + static_cast<int>(lane)) * p.sfa_row_stride;
-                const float* sfb[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    sfb[h] = p.sfb + group * p.sfb_group_stride + static_cast<long long>(min(t.n0 + h * (BLOCK_N / 2), p.n - 1) / 128) * p.sfb_n_stride;
+                // B's scales are the same for all rows: lane 4 h + i loads the one of half h and K block i of the four
+                const float* sfb = p.sfb + group * p.sfb_group_stride +
+                                   static_cast<long long>(min(t.n0 + static_cast<int>(lane / kScaleKb % 2) * (BLOCK_N / 2), p.n - 1) / 128) * p.sfb_n_stride +
+                                   (lane % kScaleKb) * p.sfb_k_stride;
                 for (int kb = 0; ok && kb < num_kb; kb += kScaleKb) {
-                    float a[4][kScaleKb], b[2][kScaleKb];
+                    float a[4][kScaleKb];
                     const bool whole = p.sf_vec && kb + kScaleKb <= num_kb;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)  // rows that are not stored need no scale: none is read for them
                         load_scales(sfa + 32 * j * p.sfa_row_stride + kb * p.sfa_k_stride, p.sfa_k_stride,
                                     static_cast<int>(lane) + 32 * j < t.rows ? num_kb - kb : 0, whole, a[j]);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) load_scales(sfb[h] + kb * p.sfb_k_stride, p.sfb_k_stride, num_kb - kb, whole, b[h]);
+                    const float b = static_cast<int>(lane % kScaleKb) < num_kb - kb ? __ldg(sfb + kb * p.sfb_k_stride) : 0.0f;
 #pragma unroll
                     for (int i = 0; i < kScaleKb; ++i) {
                         if (!ok || kb + i >= num_kb) break;
@@ -413,9 +416,11 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                         if (!ok) break;
                         float* to = reinterpret_cast<float*>(smem + L::kOffScales + slot * L::kScaleSlotBytes) + lane;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                        for (int h = 0; h < 2; ++h) {
+                            const float bh = __shfl_sync(0xffffffffu, b, h * kScaleKb + i);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) to[h * 128 + 32 * j] = a[j][i] * b[h][i];
+                            for (int j = 0; j < 4; ++j) to[h * 128 + 32 * j] = a[j][i] * bh;
+                        }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(tmem_full_bar + as);
                         if (++as == kAccums) { as = 0; phase ^= 1; }
@@ -444,8 +449,8 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
         const float* const my_scales = reinterpret_cast<const float*>(smem + L::kOffScales) + half * 128 + r;
         Sched sched(p, table);
         BlockScaledTile t;
-        // stage of the K block at hand and of the one that will use its accumulator next (kAccums K blocks later)
-        uint32_t as = 0, aphase = 0, stage = 0, next_stage = kAccums % kStages, slot = 0;
+        // K blocks so far, and the stage of the one that will use the accumulator at hand next (kAccums K blocks later)
+        uint32_t it = 0, next_stage = kAccums % kStages;
         bool ok = true;
         while (ok && sched.next(t)) {
             if (t.group < 0) continue;
@@ -455,7 +460,8 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
 #pragma unroll 1
             for (int kb = 0; kb < num_kb; ++kb) {
-                ok = mbar_wait(tmem_full_bar + as, aphase, abort_flag, kTimeoutTmemFull, kb);
+                const uint32_t as = it % kAccums;
+                ok = mbar_wait(tmem_full_bar + as, (it / kAccums) & 1, abort_flag, kTimeoutTmemFull, kb);
                 if (!ok) break;
                 tcgen05_fence_after();
                 if (warp_has_rows) {
@@ -463,7 +469,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                     const uint32_t tmem_row = tmem_half + as * kAccumCols;
                     uint32_t v[2][kChunk];
                     tmem_ld_32x32b_x16(tmem_row, v[0]);
-                    const float s = my_scales[slot * (L::kScaleSlotBytes / 4)];
+                    const float s = my_scales[(it % L::kScaleSlots) * (L::kScaleSlotBytes / 4)];
 #pragma unroll
                     for (int c = 0; c < kCols / kChunk; ++c) {
                         tmem_ld_wait();
@@ -476,12 +482,9 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                 __syncwarp();
                 if (lane == 0) {
                     give_accumulator(next_stage);                  // this warp has read the accumulator (and the scales)
-                    if (warp == 4) mbar_arrive(empty_bar + stage);  // the K block's operands have been read
                 }
-                if (++as == kAccums) { as = 0; aphase ^= 1; }
-                if (++stage == kStages) stage = 0;
+                ++it;
                 if (++next_stage == kStages) next_stage = 0;
-                if (++slot == L::kScaleSlots) slot = 0;
             }
             if (!ok) break;
             if (!warp_has_rows) continue;
