@@ -123,13 +123,13 @@ struct BlockScaledSmem {
     // warp had left K block i - 2 kAccums, the slot's last user.
     static constexpr int kScaleSlots = 2 * kAccums;
     static constexpr int kScaleSlotBytes = 2 * 128 * 4;  // [half of the tile's columns][row]
-    static constexpr int kSlabBytes = 64;                // epilogue staging: bytes of each of a warp's 32 rows
+    static constexpr int kStagingBytes = 16 * 128;       // epilogue: 16 rows x 128 bytes of each summing warp
     static constexpr int kABytes = 128 * 128;
     static constexpr int kBBytes = BLOCK_N * 128 / (kPair ? 2 : 1);
     static constexpr int kOffA = 0;
     static constexpr int kOffB = kOffA + kStages * kABytes;
     static constexpr int kOffStage = kOffB + kStages * kBBytes;
-    static constexpr int kOffScales = kOffStage + kSumWarps * 32 * kSlabBytes;
+    static constexpr int kOffScales = kOffStage + kSumWarps * kStagingBytes;
     static constexpr int kOffBar = kOffScales + kScaleSlots * kScaleSlotBytes;
     static constexpr int kNumBars = 2 * kStages + kAccums;
     static constexpr int kOffMisc = kOffBar + (kNumBars * 8 + 15) / 16 * 16;
@@ -153,11 +153,22 @@ struct BlockScaledScheduler {
     const BlockScaledParams& p;
     const int *start, *rows, *tiles_end;
     int num_n_blocks, tile, stride, sub, g;
+    uint32_t n_magic;  // tile / num_n_blocks = its product's upper half, or one less: the summing warps ask for a tile between two others
 
     __device__ BlockScaledScheduler(const BlockScaledParams& params, const int* table)
         : p(params), start(table), rows(table + kMaxCachedGroups), tiles_end(table + 2 * kMaxCachedGroups),
           num_n_blocks((params.n + BLOCK_N - 1) / BLOCK_N), tile(static_cast<int>(blockIdx.x) / (kPair ? 2 : 1)),
-          stride(static_cast<int>(gridDim.x) / (kPair ? 2 : 1)), sub(kPair ? static_cast<int>(blockIdx.x & 1) * 128 : 0), g(0) {}
+          stride(static_cast<int>(gridDim.x) / (kPair ? 2 : 1)), sub(kPair ? static_cast<int>(blockIdx.x & 1) * 128 : 0), g(0),
+          n_magic(0xffffffffu / static_cast<uint32_t>((params.n + BLOCK_N - 1) / BLOCK_N)) {}
+
+    __device__ __forceinline__ void split(int index, int& mb, int& nb) const {
+        mb = static_cast<int>(__umulhi(static_cast<uint32_t>(index), n_magic));
+        nb = index - mb * num_n_blocks;
+        while (nb >= num_n_blocks) {
+            nb -= num_n_blocks;
+            ++mb;
+        }
+    }
 
     // Rows of a group from the layout words; whatever they hold, no row at or past p.m is named.
     __device__ __forceinline__ static void group_extent(const BlockScaledParams& p, int group, int& first, int& count) {
@@ -176,10 +187,10 @@ struct BlockScaledScheduler {
 
     __device__ bool next(BlockScaledTile& t) {
         if (p.mode == kModeDense || p.mode == kModeRowIds) {
-            const int num_m_blocks = (p.m + kTileM - 1) / kTileM;
-            if (tile >= num_m_blocks * num_n_blocks) return false;
-            const int nb = tile / num_m_blocks;
-            t.row0 = (tile - nb * num_m_blocks) * kTileM + sub;
+            if (tile >= (p.m + kTileM - 1) / kTileM * num_n_blocks) return false;
+            int mb, nb;
+            split(tile, mb, nb);
+            t.row0 = mb * kTileM + sub;
             t.rows = min(128, p.m - t.row0);
             t.n0 = nb * BLOCK_N;
             t.group = p.mode == kModeDense ? 0 : __ldg(p.layout + t.row0);  // (no pairs with row ids: t.row0 < p.m)
@@ -192,10 +203,8 @@ struct BlockScaledScheduler {
         }
         g = group_of_tile(tiles_end, g, p.num_groups, tile);
         if (g >= p.num_groups) return false;
-        const int local = tile - (g == 0 ? 0 : tiles_end[g - 1]);
-        const int num_m_blocks = (rows[g] + kTileM - 1) / kTileM;
-        const int nb = local / num_m_blocks;
-        const int mb = local - nb * num_m_blocks;
+        int mb, nb;
+        split(tile - (g == 0 ? 0 : tiles_end[g - 1]), mb, nb);
         t.row0 = start[g] + mb * kTileM + sub;
         t.rows = min(128, rows[g] - mb * kTileM - sub);
         t.n0 = nb * BLOCK_N;
@@ -434,7 +443,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
         // ---------------------------------------------------------------- running sums and epilogue
         const uint32_t q = warp & 3, half = (warp - 4) >> 2;  // lane quarter of tensor memory, half of the tile's columns
         const int r = static_cast<int>(q * 32 + lane);
-        uint8_t* stage_buf = smem + L::kOffStage + (warp - 4) * (32 * L::kSlabBytes);
+        uint8_t* stage_buf = smem + L::kOffStage + (warp - 4) * L::kStagingBytes;
         // the barriers of the MMA issuer's CTA
         const uint32_t issuer_full = kPair ? map_to_cta(smem_u32(full_bar), 0) : smem_u32(full_bar);
         auto give_accumulator = [&](uint32_t to_stage) {
@@ -489,48 +498,49 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             if (!ok) break;
             if (!warp_has_rows) continue;
             const int col0 = t.n0 + static_cast<int>(half) * kCols;
-            // Store: a slab of 32 rows x 64 (or 32) bytes at a time is turned through shared memory (16-byte chunks, XOR-swizzled), so
-            // that a store instruction of the warp writes whole sectors of eight (sixteen) rows instead of 16 bytes of 32 rows.
-            constexpr int kChunks = L::kSlabBytes / 16;             // of a row of the slab
-            constexpr int kPerChunk = kF32 ? 4 : 8;                 // columns
+            // Store: 16 rows x 128 bytes at a time are turned through shared memory (16-byte chunks, XOR-swizzled): the rows' 16 lanes write them,
+            // then every store instruction of the warp writes four whole lines instead of 16 bytes of 32 rows.
+            constexpr int kPerChunk = kF32 ? 4 : 8;                              // columns in 16 bytes
+            constexpr int kChunks = kCols / kPerChunk < 8 ? kCols / kPerChunk : 8;  // of a row of the slab
             constexpr int kSlab = kChunks * kPerChunk;
-            constexpr int kSlabs = (kCols + kSlab - 1) / kSlab;
-            auto place = [&](int row, int chunk) {
-                return reinterpret_cast<uint4*>(stage_buf + row * L::kSlabBytes + ((chunk ^ ((row * L::kSlabBytes / 128) & (kChunks - 1))) << 4));
-            };
+            auto place = [&](int row, int chunk) { return reinterpret_cast<uint4*>(stage_buf + row * 128 + ((chunk ^ (row & (kChunks - 1))) << 4)); };
             const long long row_base = (p.mode == kModeMasked ? static_cast<long long>(t.group) * p.m : 0) + t.row0 + static_cast<int>(q * 32);
             const int rows_here = t.rows - static_cast<int>(q * 32);
 #pragma unroll
-            for (int s = 0; s < kSlabs; ++s) {
-                __syncwarp();
+            for (int s = 0; s < kCols / kSlab; ++s) {
 #pragma unroll
-                for (int i = 0; i < kChunks; ++i) {
-                    const int at = s * kSlab + i * kPerChunk;
-                    if (at >= kCols) continue;
-                    const float* a = acc + at;
-                    if constexpr (kF32)
-                        *place(lane, i) = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
-                    else
-                        *place(lane, i) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
-                }
-                __syncwarp();
+                for (int h = 0; h < 2; ++h) {
+                    if (h * 16 >= rows_here) continue;
+                    __syncwarp();
+                    if (static_cast<int>(lane >> 4) == h) {
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j) {
-                    const int row = static_cast<int>(lane) / kChunks + 32 / kChunks * j, chunk = static_cast<int>(lane) % kChunks;
-                    const int in_part = s * kSlab + chunk * kPerChunk;
-                    const int col = col0 + in_part;
-                    if (row >= rows_here || in_part >= kCols || col >= p.n) continue;  // n is a multiple of 8: a chunk is inside or outside
-                    const uint4 v = *place(row, chunk);
-                    const long long at = (row_base + row) * p.d_row_stride + col;
-                    if constexpr (kF32) {
-                        float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-                        if (p.c != nullptr) {
-                            const float4 c4 = *reinterpret_cast<const float4*>(p.c + (row_base + row) * p.c_row_stride + col);
-                            f = make_float4(c4.x + f.x, c4.y + f.y, c4.z + f.z, c4.w + f.w);
+                        for (int i = 0; i < kChunks; ++i) {
+                            const float* a = acc + s * kSlab + i * kPerChunk;
+                            if constexpr (kF32)
+                                *place(lane & 15, i) = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+                            else
+                                *place(lane & 15, i) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
                         }
-                        *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at) = f;
-                    } else {
-                        st_global_v4(static_cast<__nv_bfloat16*>(p.d) + at, v.x, v.y, v.z, v.w);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < kChunks / 2; ++j) {
+                        constexpr int kRowsPer = 32 / kChunks;
+                        const int row = static_cast<int>(lane) / kChunks + kRowsPer * j, chunk = static_cast<int>(lane) % kChunks;
+                        const int col = col0 + s * kSlab + chunk * kPerChunk;
+                        if (h * 16 + row >= rows_here || col >= p.n) continue;  // n is a multiple of 8: a chunk is inside or outside
+                        const uint4 v = *place(row, chunk);
+                        const long long at = (row_base + h * 16 + row) * p.d_row_stride + col;
+                        if constexpr (kF32) {
+                            float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+                            if (p.c != nullptr) {
+                                const float4 c4 = *reinterpret_cast<const float4*>(p.c + (row_base + h * 16 + row) * p.c_row_stride + col);
+                                f = make_float4(c4.x + f.x, c4.y + f.y, c4.z + f.z, c4.w + f.w);
+                            }
+                            *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at) = f;
+                        } else {
+                            st_global_v4(static_cast<__nv_bfloat16*>(p.d) + at, v.x, v.y, v.z, v.w);
+                        }
                     }
                 }
             }
