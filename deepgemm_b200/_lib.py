@@ -73,7 +73,7 @@ _SIGNATURES = {
     'dgb200_moe_dispatch_plan_noalloc': [_ptr, _i32, _i32, _i32, _i32, _ptr, _ptr, _ptr, _ptr],
     'dgb200_set_mega_moe_stage_events': [_ptr, _i32],
     'dgb200_ep_plan_with_guest_experts': [_ptr, _i32, _i32, _i32, _i32, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr],
-    'dgb200_fp8_block_scaled_gemm': [_ptr, _ptr],
+    'dgb200_fp8_block_scaled_gemm': [ctypes.c_char_p, _ptr],  # the argument struct, packed (block_scaled.py)
     'dgb200_per_token_cast_to_fp8_f32_scales': [_ptr, _i64, _i32, _i32, _i32, _ptr, _i64, _ptr, _i64, _ptr],
     'dgb200_per_block_cast_to_fp8': [_ptr, _i64, _i64, _i32, _i32, _i32, _i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr],
     'dgb200_moe_dispatch_plan_workspace_bytes': [_i32, _i32, _i32],
@@ -101,16 +101,6 @@ class MegaMoeArgs(ctypes.Structure):
                                        'hidden', 'intermediate_hidden')] + \
         [('activation_clamp', ctypes.c_float), ('fast_math', ctypes.c_int32), ('num_guest_experts', ctypes.c_int32)] + \
         [(n, ctypes.c_void_p) for n in ('peer_l1_w', 'peer_l1_w_sf', 'peer_l2_w', 'peer_l2_w_sf')]
-
-
-class BlockScaledGemmArgs(ctypes.Structure):
-    """dgb200_fp8_block_scaled_gemm_args of include/dgb200.h, field for field."""
-    _fields_ = [('struct_size', ctypes.c_size_t)] + \
-        [(n, ctypes.c_void_p) for n in ('a', 'sfa', 'b', 'sfb', 'd', 'c', 'layout')] + \
-        [(n, ctypes.c_int64) for n in ('sfa_group_stride', 'sfa_row_stride', 'sfa_k_stride', 'sfb_group_stride', 'sfb_n_stride', 'sfb_k_stride',
-                                       'd_row_stride', 'c_row_stride')] + \
-        [(n, ctypes.c_int32) for n in ('m', 'n', 'k', 'num_groups', 'layout_kind', 'alignment', 'store_padding', 'expected_m', 'b_mn_major',
-                                       'd_is_fp32')]
 
 
 def exported_symbols():

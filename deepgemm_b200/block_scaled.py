@@ -1,32 +1,42 @@
 """FP8 GEMMs whose operands carry FP32 scales, one per 1 x 128 values of a and per 128 x 128 of b: what the entry points of
 ``gemm`` do with float32 scales and ``disable_ue8m0_cast=True`` (the reference's FP32-scale kernels, csrc/apis/gemm.hpp:73-124,
 :166-297, exist for the previous architecture only)."""
-import ctypes
+import struct
 
 import torch
 
 from . import _lib
 from .layout import check_sf_layout
 
+# dgb200_fp8_block_scaled_gemm_args of include/dgb200.h: size, seven pointers, eight strides, ten ints. Packed by hand: a
+# ctypes.Structure takes 6 us to fill, a third of what a small call takes on the host.
+_ARGS = struct.Struct('@N7P8q10i')
+
 LAYOUT_ROW_IDS, LAYOUT_PSUM, LAYOUT_MASKED, LAYOUT_DENSE = range(4)
 
 
-def check_same_device(*tensors):
+def check_same_device(first, *tensors):
     """Pointers of one call go to one device."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f'all tensors of a call must be on one device, got {sorted(map(str, devices))}')
+    index = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f'all tensors of a call must be on one device, got {first.device} and {t.device}')
+
+
+def span(t: torch.Tensor):
+    """First byte and one past the last of a tensor's memory."""
+    start = t.data_ptr()
+    if t.is_contiguous():
+        return start, start + t.nbytes
+    if t.numel() == 0:
+        return start, start
+    return start, start + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory spans of two tensors meet (strided tensors: from the first to the last byte)."""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    if a.numel() == 0 or b.numel() == 0:
-        return False
+    """Whether the memory spans of two tensors meet."""
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    return a0 < b1 and b0 < a1 and a0 < a1 and b0 < b1
 
 
 def wanted(a_sf: torch.Tensor, b_sf: torch.Tensor, disable_ue8m0_cast: bool) -> bool:
@@ -91,17 +101,18 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
         if not same and (overlap(c, d) or c.stride(-1) != 1 or c.stride(-2) % 4 != 0 or c.stride(-2) < n or c.data_ptr() % 16 != 0):
             c = c.contiguous() if not overlap(c, d) else c.clone(memory_format=torch.contiguous_format)
     check_same_device(a_q, a_sf, b_q, b_sf, d, c, layout)
-    if any(overlap(d, t) for t in (a_q, a_sf, b_q, b_sf)):
-        raise RuntimeError('d must not overlap an operand')
     if m == 0:
         return
-    p = lambda t: t.data_ptr() if t is not None else None
-    args = _lib.BlockScaledGemmArgs(
-        struct_size=ctypes.sizeof(_lib.BlockScaledGemmArgs), a=p(a_q), sfa=p(a_sf), b=p(b_q), sfb=p(b_sf), d=p(d), c=p(c), layout=p(layout),
-        sfa_group_stride=a_sf.stride(0) if masked else 0, sfa_row_stride=a_sf.stride(-2), sfa_k_stride=a_sf.stride(-1),
-        sfb_group_stride=0 if dense else b_sf.stride(0), sfb_n_stride=b_sf.stride(-2), sfb_k_stride=b_sf.stride(-1),
-        d_row_stride=row_stride, c_row_stride=(c.stride(-2) if m > 1 else max(c.stride(-2), n)) if c is not None else 0,
-        m=m, n=n, k=k, num_groups=groups, layout_kind=layout_kind, alignment=alignment, store_padding=int(bool(store_padding)),
-        expected_m=int(expected_m), b_mn_major=int(b_mn_major), d_is_fp32=int(d.dtype == torch.float32))
+    d0, d1 = span(d)
+    for t in (a_q, a_sf, b_q, b_sf):
+        t0, t1 = span(t)
+        if t0 < d1 and d0 < t1:
+            raise RuntimeError('d must not overlap an operand')
+    args = _ARGS.pack(
+        _ARGS.size, a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(), d.data_ptr(), c.data_ptr() if c is not None else 0,
+        layout.data_ptr() if layout is not None else 0, a_sf.stride(0) if masked else 0, a_sf.stride(-2), a_sf.stride(-1),
+        0 if dense else b_sf.stride(0), b_sf.stride(-2), b_sf.stride(-1), row_stride,
+        (c.stride(-2) if m > 1 else max(c.stride(-2), n)) if c is not None else 0, m, n, k, groups, layout_kind, alignment,
+        int(bool(store_padding)), int(expected_m), int(b_mn_major), int(d.dtype == torch.float32))
     with _lib.on_device(d.device):
-        _lib.check(_lib.lib().dgb200_fp8_block_scaled_gemm(ctypes.byref(args), _lib.current_stream_ptr()))
+        _lib.check(_lib.lib().dgb200_fp8_block_scaled_gemm(args, _lib.current_stream_ptr()))

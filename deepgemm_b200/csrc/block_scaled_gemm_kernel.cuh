@@ -147,6 +147,7 @@ struct BlockScaledTile {
 
 // Walks the output tiles. Groups come from the table that the prologue puts into shared memory: start row, rows to
 // compute and running tile count of each.
+// `ctas`: CTAs that share a tile (a pair, or a cluster that splits the tile's K).
 template <int BLOCK_N, bool kPair>
 struct BlockScaledScheduler {
     static constexpr int kTileM = kPair ? 256 : 128;
@@ -155,10 +156,10 @@ struct BlockScaledScheduler {
     int num_n_blocks, tile, stride, sub, g;
     uint32_t n_magic;  // tile / num_n_blocks = its product's upper half, or one less: the summing warps ask for a tile between two others
 
-    __device__ BlockScaledScheduler(const BlockScaledParams& params, const int* table)
+    __device__ BlockScaledScheduler(const BlockScaledParams& params, const int* table, int ctas)
         : p(params), start(table), rows(table + kMaxCachedGroups), tiles_end(table + 2 * kMaxCachedGroups),
-          num_n_blocks((params.n + BLOCK_N - 1) / BLOCK_N), tile(static_cast<int>(blockIdx.x) / (kPair ? 2 : 1)),
-          stride(static_cast<int>(gridDim.x) / (kPair ? 2 : 1)), sub(kPair ? static_cast<int>(blockIdx.x & 1) * 128 : 0), g(0),
+          num_n_blocks((params.n + BLOCK_N - 1) / BLOCK_N), tile(static_cast<int>(blockIdx.x) / ctas),
+          stride(static_cast<int>(gridDim.x) / ctas), sub(kPair ? static_cast<int>(blockIdx.x & 1) * 128 : 0), g(0),
           n_magic(0xffffffffu / static_cast<uint32_t>((params.n + BLOCK_N - 1) / BLOCK_N)) {}
 
     __device__ __forceinline__ void split(int index, int& mb, int& nb) const {
@@ -216,7 +217,10 @@ struct BlockScaledScheduler {
 
 constexpr int kRegsBsControl = 72, kRegsBsSum = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
 
-template <int BLOCK_N, int kStages, bool kF32, bool kPair>
+// kSplitK (dense form): the CTAs of a cluster (2, 4 or 8) share one tile and take a part of its K blocks each; every CTA leaves its sums in its
+// own shared memory (the operand ring is done with), then the cluster adds them up, rank by rank in a fixed order. For problems
+// with so few tiles that most SMs would idle while a few pull all of B.
+template <int BLOCK_N, int kStages, bool kF32, bool kPair, bool kSplitK = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                                 const __grid_constant__ BlockScaledParams p) {
@@ -230,6 +234,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     constexpr int kCols = BLOCK_N / (kSumWarps / 4);  // columns a thread sums
     static_assert(BLOCK_N == 32 || BLOCK_N == 64 || BLOCK_N == 128 || BLOCK_N == 256, "tile width");
     static_assert(!kPair || BLOCK_N == 256, "pairs work on 256 x 256 tiles");
+    static_assert(!kSplitK || (!kPair && kStages * (L::kABytes + L::kBBytes) >= 128 * BLOCK_N * 4), "the operand ring holds the FP32 tile");
     static_assert(L::kDynamicBytes <= 232448, "shared memory budget");
 
     extern __shared__ uint8_t smem_raw[];
@@ -299,7 +304,14 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     if constexpr (kPair) cluster_sync_all();
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_ptr_smem;
-    const int num_kb = (p.k + 127) / 128;
+    // this CTA's K blocks; parts are whole groups of kScaleKb, and the host leaves none empty
+    const int tile_ctas = kPair ? 2 : (kSplitK ? static_cast<int>(cluster_num_ctas()) : 1);
+    int first_kb = 0, num_kb = (p.k + 127) / 128;  // [first_kb, num_kb)
+    if constexpr (kSplitK) {
+        const int rank = static_cast<int>(cluster_cta_rank()), units = (num_kb + kScaleKb - 1) / kScaleKb;
+        first_kb = units * rank / tile_ctas * kScaleKb;
+        num_kb = min(units * (rank + 1) / tile_ctas * kScaleKb, num_kb);
+    }
 
     // In a pair the leader's loaders announce the bytes of both CTAs (their loads are alike), the other CTA's only arrive.
     auto stage_arrive = [&](uint32_t stage, uint32_t bytes) {
@@ -321,13 +333,13 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             // ------------------------------------------------------------ loaders: A (warp 0) and B (warp 3)
             const bool is_a = warp == 0;
             const bool elected = elect_one();
-            Sched sched(p, table);
+            Sched sched(p, table, tile_ctas);
             BlockScaledTile t;
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             while (ok && sched.next(t)) {
                 if (t.group < 0) continue;
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = first_kb; kb < num_kb; ++kb) {
                     ok = mbar_wait(empty_bar + stage, phase ^ 1, abort_flag, kTimeoutEmpty, kb);
                     if (!ok) break;
                     if (elected) {
@@ -356,7 +368,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             // The summing warps leave this one few issue slots, and a K block is only 512 cycles (256 for a 128-wide tile) of MMAs: its loop holds
             // few instructions. Descriptors are one word each, moved on by additions, and there is one barrier to wait for.
             const bool elected = elect_one();
-            Sched sched(p, table);
+            Sched sched(p, table, tile_ctas);
             BlockScaledTile t;
             const bool b_mn = BLOCK_N >= 128 && p.b_mn_major;
             const uint32_t idesc = make_idesc_e4m3_f32(128 * kCtas, BLOCK_N) | (b_mn ? (1u << 16) : 0u);
@@ -368,7 +380,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             while (ok && sched.next(t)) {
                 if (t.group < 0) continue;
 #pragma unroll 1
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = first_kb; kb < num_kb; ++kb) {
                     ok = mbar_wait(full_bar + stage, phase, abort_flag, kTimeoutFull, kb);
                     if (!ok) break;
                     tcgen05_fence_after();
@@ -398,7 +410,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             // ------------------------------------------------------------ scales: sfa[row] * sfb[column block]
             // The loads of four K blocks are under way together, well ahead of their use; read by the summing warps
             // themselves, one K block ahead, their latency was a fifth of the kernel.
-            Sched sched(p, table);
+            Sched sched(p, table, tile_ctas);
             BlockScaledTile t;
             uint32_t as = 0, phase = 0, slot = 0;
             bool ok = true;
@@ -410,7 +422,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                 const float* sfb = p.sfb + group * p.sfb_group_stride +
                                    static_cast<long long>(min(t.n0 + static_cast<int>(lane / kScaleKb % 2) * (BLOCK_N / 2), p.n - 1) / 128) * p.sfb_n_stride +
                                    (lane % kScaleKb) * p.sfb_k_stride;
-                for (int kb = 0; ok && kb < num_kb; kb += kScaleKb) {
+                for (int kb = first_kb; ok && kb < num_kb; kb += kScaleKb) {
                     float a[4][kScaleKb];
                     const bool whole = p.sf_vec && kb + kScaleKb <= num_kb;
 #pragma unroll
@@ -456,7 +468,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
         }
         const uint32_t tmem_half = tmem_base + ((q * 32u) << 16) + half * kCols;
         const float* const my_scales = reinterpret_cast<const float*>(smem + L::kOffScales) + half * 128 + r;
-        Sched sched(p, table);
+        Sched sched(p, table, tile_ctas);
         BlockScaledTile t;
         // K blocks so far, and the stage of the one that will use the accumulator at hand next (kAccums K blocks later)
         uint32_t it = 0, next_stage = kAccums % kStages;
@@ -468,7 +480,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
 #pragma unroll
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
 #pragma unroll 1
-            for (int kb = 0; kb < num_kb; ++kb) {
+            for (int kb = first_kb; kb < num_kb; ++kb) {
                 const uint32_t as = it % kAccums;
                 ok = mbar_wait(tmem_full_bar + as, (it / kAccums) & 1, abort_flag, kTimeoutTmemFull, kb);
                 if (!ok) break;
@@ -497,6 +509,15 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             }
             if (!ok) break;
             if (!warp_has_rows) continue;
+            if constexpr (kSplitK) {
+                // All MMAs of this CTA are complete and with them its loads: the ring is free. 16-byte chunks, XOR-swizzled.
+                uint8_t* mine = smem + r * (BLOCK_N * 4);
+#pragma unroll
+                for (int i = 0; i < kCols / 4; ++i)
+                    *reinterpret_cast<float4*>(mine + (((static_cast<int>(half) * (kCols / 4) + i) ^ (r & 7)) << 4)) =
+                        make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+                continue;  // the cluster adds and stores below
+            }
             const int col0 = t.n0 + static_cast<int>(half) * kCols;
             // Store: 16 rows x 128 bytes at a time are turned through shared memory (16-byte chunks, XOR-swizzled): the rows' 16 lanes write them,
             // then every store instruction of the warp writes four whole lines instead of 16 bytes of 32 rows.
@@ -545,6 +566,57 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                 }
             }
         }
+    }
+
+    if constexpr (kSplitK) {
+        // A CTA that gave up on a wait leaves zeros or stale bytes in its part; the error is in the status block.
+        __syncwarp();
+        cluster_sync_all();
+        Sched sched(p, table, tile_ctas);
+        BlockScaledTile t;
+        if (sched.next(t)) {
+            constexpr int kOct = BLOCK_N / 8;  // 8 columns per thread and step
+            const int items = max(t.rows, 0) * kOct;
+            for (int i = static_cast<int>(cluster_cta_rank() * kGemmThreads + threadIdx.x); i < items; i += tile_ctas * kGemmThreads) {
+                const int row = i / kOct, oct = i % kOct, col = t.n0 + oct * 8;
+                if (col >= p.n) continue;
+                const uint32_t at_row = smem_u32(smem + row * (BLOCK_N * 4));
+                float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                for (int c0 = 0; c0 < tile_ctas; c0 += 2) {  // two ranks' loads in flight
+                    float4 f[2][2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            f[c][h] = ld_cluster_f4(map_to_cta(at_row + (((oct * 2 + h) ^ (row & 7)) << 4), static_cast<uint32_t>(c0 + c)));
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            v[4 * h] += f[c][h].x;
+                            v[4 * h + 1] += f[c][h].y;
+                            v[4 * h + 2] += f[c][h].z;
+                            v[4 * h + 3] += f[c][h].w;
+                        }
+                }
+                const long long at = static_cast<long long>(t.row0 + row) * p.d_row_stride + col;
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float4 o = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+                        if (p.c != nullptr) {
+                            const float4 c4 = *reinterpret_cast<const float4*>(p.c + static_cast<long long>(t.row0 + row) * p.c_row_stride + col + 4 * h);
+                            o = make_float4(c4.x + o.x, c4.y + o.y, c4.z + o.z, c4.w + o.w);
+                        }
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.d) + at + 4 * h) = o;
+                    }
+                } else {
+                    st_global_v4(static_cast<__nv_bfloat16*>(p.d) + at, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                                 pack_bf16x2(v[6], v[7]));
+                }
+            }
+        }
+        cluster_sync_all();  // nobody leaves while others read its shared memory
     }
 
     // ---------------------------------------------------------------- teardown

@@ -48,6 +48,64 @@ int launch_block_scaled(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const 
     return 0;
 }
 
+// The split-K form: clusters of `split` CTAs, one for each of `tiles` tiles. `max_clusters` receives how many of them the device runs at
+// the same time (asked once per form, size and device; with `dry` nothing is launched).
+template <bool kF32>
+int launch_block_scaled_split(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const BlockScaledParams& p, int tiles, int split, bool dry,
+                              int* max_clusters, cudaStream_t stream) {
+    using L = BlockScaledSmem<128, 6, false>;
+    auto kernel = dgb200_block_scaled_gemm_kernel<128, 6, kF32, false, true>;
+    static std::atomic<int> done[64] = {}, active[64][4] = {};  // [device][log2 split]; 0 = not asked yet
+    if (const int rc = allow_dynamic_smem(kernel, L::kDynamicBytes, done)) return rc;
+    int dev = 0;
+    DGB_CUDA(cudaGetDevice(&dev));
+    std::atomic<int>& known = active[dev][split == 2 ? 1 : (split == 4 ? 2 : 3)];
+    int clusters = known.load(std::memory_order_acquire);
+    if (clusters == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(split));
+        cfg.blockDim = dim3(kGemmThreads);
+        cfg.dynamicSmemBytes = L::kDynamicBytes;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        DGB_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg));
+        known.store(clusters > 0 ? clusters : -1, std::memory_order_release);
+    }
+    *max_clusters = std::max(clusters, 0);
+    if (dry) return 0;
+    DGB_CUDA(launch_kernel_in_clusters(split, kernel, dim3(static_cast<unsigned>(tiles * split)), dim3(kGemmThreads), L::kDynamicBytes, stream,
+                                       use_pdl(), tm_a, tm_b, p));
+    return 0;
+}
+
+// CTAs per tile of a dense GEMM (1: no split): the largest of 8, 4 and 2 for which all clusters run at once and every part keeps at least 8
+// (12 where more than 64 rows have to be added up) K blocks. Device time of calls back to back, no split (the narrowest tiles) -> split
+// (us): 7 x 4096 x 7168 15.7 -> 11.0 (4), 1 x 7168 x 2048 10.2 -> 7.8 (2), 33 x 1536 x 7168 15.1 -> 10.5 (4; 8: 11.1), 256 x 4096 x 7168 27.6 ->
+// 15.7 (2), 128 x 7168 x 16384 58.8 -> 29.4 (2). With less K it does not pay: 128 x 4096 x 2048 7.0 -> 9.6 (2), 11.7 (4); 128 x 4096 x
+// 1024 5.2 -> 8.5 (2).
+int block_scaled_split(long long tiles, int rows, int num_kb, bool f32, int sms, int* split) {
+    *split = 1;
+    if (tuning().split_k == 0) return 0;
+    const int units = (num_kb + kScaleKb - 1) / kScaleKb;
+    for (const int s : {8, 4, 2}) {
+        if (tuning().split_k > 0 ? s != tuning().split_k || units < s : units < (rows > 64 ? 3 : 2) * s) continue;
+        if (tiles * s > sms) continue;
+        int clusters = 0;
+        const CUtensorMap none{};
+        const int rc = f32 ? launch_block_scaled_split<true>(none, none, BlockScaledParams{}, 0, s, true, &clusters, nullptr)
+                           : launch_block_scaled_split<false>(none, none, BlockScaledParams{}, 0, s, true, &clusters, nullptr);
+        if (rc) return rc;
+        if (tiles > clusters) continue;
+        *split = s;
+        return 0;
+    }
+    return 0;
+}
+
 int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream_t stream) {
     const bool dense = a.layout_kind == DGB200_LAYOUT_DENSE, masked = a.layout_kind == DGB200_LAYOUT_MASKED;
     const bool row_ids = a.layout_kind == DGB200_LAYOUT_ROW_IDS, psum = a.layout_kind == DGB200_LAYOUT_PSUM;
@@ -110,9 +168,17 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
         const int narrowest = a.b_mn_major ? 128 : 32;
         while (block_n > narrowest && tiles_at(block_n) < sms) block_n /= 2;
     }
-    const long long rows256 = groups * ((expected + 255) / 256);
+    int split = 1;
+    if (dense && tuning().block_n == 0) {
+        if (const int rc = block_scaled_split(tiles_at(128), a.m, (a.k + 127) / 128, a.d_is_fp32 != 0, sms, &split)) return rc;
+        if (split > 1) block_n = 128;
+    }
+    // Pairs load 32 KB per SM and K block instead of 48. Single CTAs -> pairs (us): dense 4096 x 4096 x 7168 125 -> 117, 8192 x 7168 x 4096
+    // 255 -> 226. With groups half a pair tile is lost on every second one: N 4096, K 7168, 32 groups of 247 rows 323 -> 371, 8 of
+    // 900 239 -> 250, 4 of 2000 248 -> 250.
+    const long long pair_tiles = groups * ((expected + 255) / 256) * ((a.n + 255) / 256);
     const bool pair = !row_ids && block_n == 256 && sms >= 2 && tuning().pair != 0 &&
-                      (tuning().pair == 1 || (expected > 128 && rows256 * ((a.n + 255) / 256) * 2 >= sms));
+                      (tuning().pair == 1 || (expected > (dense ? 128 : 2048) && pair_tiles * 2 >= sms));
     p.a_box_rows = 128;
     if (!pair && (dense || masked) && a.m < 128) p.a_box_rows = (a.m + 7) / 8 * 8;
 
@@ -128,6 +194,12 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     // upper bound of the tiles: a group may end in a short one
     const long long max_tiles = ((masked ? groups * ((a.m + 127ll) / 128) : (a.m + 127ll) / 128 + (psum ? groups : 0))) * ((a.n + block_n - 1) / block_n);
     DGB_REQUIRE(max_tiles < (1ll << 31), "too many output tiles");
+    if (split > 1) {
+        int clusters = 0;
+        const int tiles = static_cast<int>(tiles_at(128));
+        return a.d_is_fp32 ? launch_block_scaled_split<true>(tm_a, tm_b, p, tiles, split, false, &clusters, stream)
+                           : launch_block_scaled_split<false>(tm_a, tm_b, p, tiles, split, false, &clusters, stream);
+    }
     int grid = static_cast<int>(std::min<long long>(sms, max_tiles));
     if (pair) grid = std::max(2, std::min(sms / 2 * 2, static_cast<int>((max_tiles + 1) / 2 * 2)));
 #define DGB_BS_LAUNCH(BN, STAGES, PAIR)                                                            \

@@ -15,10 +15,15 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .block_scaled import check_same_device, overlap
+from .block_scaled import check_same_device, span
 from .runtime import get_mk_alignment_for_contiguous_layout
 
 _MAX_TOPK, _MAX_EXPERTS = 32, 1024
+
+
+def _capacity(entries: int, experts: int, alignment: int) -> int:
+    step = max(alignment, 8)
+    return -(-(entries + min(experts, entries) * (alignment - 1)) // step) * step
 
 
 class MoeDispatchPlan(NamedTuple):
@@ -34,32 +39,40 @@ class MoeDispatchPlan(NamedTuple):
 
     @property
     def capacity(self) -> int:
-        """Rows that hold the sorted tokens however they are routed (known without reading the plan back), a multiple of 8 and of the
-        alignment where that is a power of two."""
-        entries = self.dest_row.numel()
-        step = max(self.alignment, 8)
-        return -(-(entries + min(self.num_experts, entries) * (self.alignment - 1)) // step) * step
+        """Rows that hold the sorted tokens however they are routed (known without reading the plan back), rounded up to a multiple
+        of 8 or of the alignment, whichever is larger."""
+        return _capacity(self.dest_row.numel(), self.num_experts, self.alignment)
 
 
 def _check_plan(plan: MoeDispatchPlan):
-    for t, dims, name in ((plan.dest_row, 2, 'dest_row'), (plan.expert_start, 1, 'expert_start'), (plan.expert_end, 1, 'expert_end')):
-        if not (t.is_cuda and t.dtype == torch.int32 and t.dim() == dims and t.is_contiguous()):
-            raise RuntimeError(f'plan.{name} must be a contiguous {dims}-D CUDA int32 tensor')
-    if not 1 <= plan.dest_row.size(1) <= _MAX_TOPK:
+    """Returns (tokens, topk, experts, capacity)."""
+    dest, start, end, alignment = plan
+    if not (dest.is_cuda and dest.dtype == torch.int32 and dest.dim() == 2 and dest.is_contiguous()):
+        raise RuntimeError('plan.dest_row must be a contiguous CUDA int32 [tokens, topk] tensor')
+    if not (end.is_cuda and end.dtype == torch.int32 and end.dim() == 1 and end.is_contiguous()):
+        raise RuntimeError('plan.expert_end must be a contiguous CUDA int32 [experts] tensor')
+    tokens, topk = dest.shape
+    if not 1 <= topk <= _MAX_TOPK:
         raise RuntimeError(f'num_topk must be in [1, {_MAX_TOPK}]')
-    if not 1 <= plan.num_experts <= _MAX_EXPERTS or plan.expert_start.numel() != plan.num_experts:
+    experts = end.numel()
+    if not 1 <= experts <= _MAX_EXPERTS or start.shape != end.shape:
         raise RuntimeError(f'the plan must hold 1 to {_MAX_EXPERTS} experts')
-    if plan.alignment < 1:
+    if alignment < 1:
         raise RuntimeError('the alignment must be positive')
+    return tokens, topk, experts, _capacity(tokens * topk, experts, alignment)
 
 
 def _check_rows(t: torch.Tensor, rows: Optional[int], width: Optional[int], dtypes, name: str):
-    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes and (t.stride(1) == 1 or t.size(1) == 1)):
-        raise RuntimeError(f'{name} must be a 2-D CUDA tensor with unit inner stride, one of {", ".join(map(str, dtypes))}')
-    if (rows is not None and t.size(0) != rows) or (width is not None and t.size(1) != width) or t.size(1) == 0:
-        raise RuntimeError(f'{name} has shape {tuple(t.shape)}, expected ({rows if rows is not None else "any"}, '
+    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes):
+        raise RuntimeError(f'{name} must be a 2-D CUDA tensor, one of {", ".join(map(str, dtypes))}')
+    height, columns = t.shape
+    row_stride, inner = t.stride()
+    if inner != 1 and columns != 1:
+        raise RuntimeError(f'{name} must have unit inner stride')
+    if (rows is not None and height != rows) or (width is not None and columns != width) or columns == 0:
+        raise RuntimeError(f'{name} has shape {(height, columns)}, expected ({rows if rows is not None else "any"}, '
                            f'{width if width is not None else "at least 1"})')
-    if t.size(0) > 1 and t.stride(0) < t.size(1):
+    if height > 1 and row_stride < columns:
         raise RuntimeError(f'rows of {name} must not overlap')
 
 
@@ -69,8 +82,12 @@ def _stride(t: torch.Tensor) -> int:
 
 
 def _check_out(out: torch.Tensor, inputs, name='out'):
-    if any(t is not None and overlap(out, t) for t in inputs):
-        raise RuntimeError(f'{name} must not overlap an input')
+    start, end = span(out)
+    for t in inputs:
+        if t is not None:
+            t_start, t_end = span(t)
+            if t_start < end and start < t_end and t_start < t_end and start < end:
+                raise RuntimeError(f'{name} must not overlap an input')
 
 
 def moe_dispatch_plan(topk_idx: torch.Tensor, num_experts: int, alignment: Optional[int] = None) -> MoeDispatchPlan:
@@ -90,12 +107,12 @@ def moe_dispatch_plan(topk_idx: torch.Tensor, num_experts: int, alignment: Optio
     lib = _lib.lib()
     workspace_bytes = lib.dgb200_moe_dispatch_plan_workspace_bytes(tokens, topk, num_experts)
     with _lib.on_device(topk_idx.device):
-        words = torch.empty(2 * num_experts + tokens * topk + workspace_bytes // 4, dtype=torch.int32, device=topk_idx.device)
-        start, end = words[:num_experts], words[num_experts:2 * num_experts]
-        dest = words[2 * num_experts:2 * num_experts + tokens * topk].view(tokens, topk)
+        dest = torch.empty((tokens, topk), dtype=torch.int32, device=topk_idx.device)
+        start, end = torch.empty((2, num_experts), dtype=torch.int32, device=topk_idx.device).unbind(0)
+        workspace = torch.empty(workspace_bytes, dtype=torch.int8, device=topk_idx.device) if workspace_bytes else None
         _lib.check(lib.dgb200_moe_dispatch_plan(
             topk_idx.data_ptr(), tokens, topk, num_experts, alignment, dest.data_ptr(), start.data_ptr(), end.data_ptr(),
-            words.data_ptr() + 4 * (2 * num_experts + tokens * topk) if workspace_bytes else None, _lib.current_stream_ptr()))
+            workspace.data_ptr() if workspace is not None else None, _lib.current_stream_ptr()))
     return MoeDispatchPlan(dest, start, end, alignment)
 
 
@@ -104,8 +121,8 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], plan:
     (float8_e4m3fn [tokens, hidden], float32 scales [tokens, blocks]) of a quantiser, then so is the result. The rows between a
     segment's end and its aligned end become zero (``zero_padding``; the K-grouped GEMMs need that, the m-grouped ones do
     not); rows behind the last segment are left as they are. ``out``: a buffer (or pair) of at least ``plan.capacity`` rows."""
-    _check_plan(plan)
-    tokens = plan.dest_row.size(0)
+    tokens, topk, experts, capacity = _check_plan(plan)
+    dest, end = plan.dest_row, plan.expert_end
     pair = isinstance(x, tuple)
     if pair and (len(x) != 2 or (out is not None and (not isinstance(out, tuple) or len(out) != 2))):
         raise RuntimeError('x and out must both be pairs (rows, scales), or both tensors')
@@ -113,28 +130,25 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], plan:
     _check_rows(q, tokens, None, (torch.float8_e4m3fn,) if pair else (torch.bfloat16, torch.float32), 'x')
     if pair:
         _check_rows(sf, tokens, None, (torch.float32,), 'the scales')
-    if out is None:
-        with _lib.on_device(q.device):
-            rows = torch.empty((plan.capacity, q.size(1)), dtype=q.dtype, device=q.device)
-            rows_sf = torch.empty((plan.capacity, sf.size(1)), dtype=torch.float32, device=q.device) if pair else None
-    else:
-        rows, rows_sf = out if pair else (out, None)
-        _check_rows(rows, None, q.size(1), (q.dtype,), 'out')
-        if pair:
-            _check_rows(rows_sf, rows.size(0), sf.size(1), (torch.float32,), 'the scales of out')
-        if rows.size(0) < plan.capacity:
-            raise RuntimeError(f'out needs at least plan.capacity ({plan.capacity}) rows, got {rows.size(0)}')
-        _check_out(rows, (q, sf, plan.dest_row, plan.expert_end))
-        if pair:
-            _check_out(rows_sf, (q, sf, rows, plan.dest_row, plan.expert_end), 'the scales of out')
-    check_same_device(q, sf, rows, rows_sf, plan.dest_row, plan.expert_end)
-    size = q.element_size()
     with _lib.on_device(q.device):
+        if out is None:
+            rows = torch.empty((capacity, q.size(1)), dtype=q.dtype, device=q.device)
+            rows_sf = torch.empty((capacity, sf.size(1)), dtype=torch.float32, device=q.device) if pair else None
+        else:
+            rows, rows_sf = out if pair else (out, None)
+            _check_rows(rows, None, q.size(1), (q.dtype,), 'out')
+            if rows.size(0) < capacity:
+                raise RuntimeError(f'out needs at least plan.capacity ({capacity}) rows, got {rows.size(0)}')
+            _check_out(rows, (q, sf, dest, end))
+            if pair:
+                _check_rows(rows_sf, rows.size(0), sf.size(1), (torch.float32,), 'the scales of out')
+                _check_out(rows_sf, (q, sf, rows, dest, end), 'the scales of out')
+        check_same_device(q, sf, rows, rows_sf, dest, end)
+        size = q.element_size()
         _lib.check(_lib.lib().dgb200_moe_permute(
             q.data_ptr(), q.size(1) * size, _stride(q) * size, rows.data_ptr(), _stride(rows) * size, sf.data_ptr() if pair else None,
             sf.size(1) if pair else 0, _stride(sf) if pair else 0, rows_sf.data_ptr() if pair else None, _stride(rows_sf) if pair else 0,
-            plan.dest_row.data_ptr(), plan.expert_end.data_ptr(), tokens, plan.dest_row.size(1), plan.num_experts, plan.alignment,
-            rows.size(0), int(zero_padding), _lib.current_stream_ptr()))
+            dest.data_ptr(), end.data_ptr(), tokens, topk, experts, plan.alignment, rows.size(0), int(zero_padding), _lib.current_stream_ptr()))
     return (rows, rows_sf) if pair else rows
 
 
@@ -143,20 +157,18 @@ def moe_unpermute(rows: torch.Tensor, plan: MoeDispatchPlan, topk_weights: Optio
     """``y[t] = sum_k topk_weights[t, k] * rows[plan.dest_row[t, k]]``, summed in ascending k in FP32 and rounded once; masked
     entries add nothing. ``rows`` bfloat16 or float32 [>= plan.capacity, hidden]; ``topk_weights`` float32 [tokens, topk] or None
     (every weight one); returns [tokens, hidden] of the type of ``rows``."""
-    _check_plan(plan)
-    tokens, topk = plan.dest_row.shape
+    tokens, topk, experts, capacity = _check_plan(plan)
     _check_rows(rows, None, None, (torch.bfloat16, torch.float32), 'rows')
-    if rows.size(0) < plan.capacity:
-        raise RuntimeError(f'rows must hold plan.capacity ({plan.capacity}) rows, got {rows.size(0)}')
+    if rows.size(0) < capacity:
+        raise RuntimeError(f'rows must hold plan.capacity ({capacity}) rows, got {rows.size(0)}')
     _check_weights(topk_weights, plan)
-    if out is None:
-        with _lib.on_device(rows.device):
-            out = torch.empty((tokens, rows.size(1)), dtype=rows.dtype, device=rows.device)
-    else:
-        _check_rows(out, tokens, rows.size(1), (rows.dtype,), 'out')
-        _check_out(out, (rows, topk_weights, plan.dest_row))
-    check_same_device(rows, out, topk_weights, plan.dest_row)
     with _lib.on_device(rows.device):
+        if out is None:
+            out = torch.empty((tokens, rows.size(1)), dtype=rows.dtype, device=rows.device)
+        else:
+            _check_rows(out, tokens, rows.size(1), (rows.dtype,), 'out')
+            _check_out(out, (rows, topk_weights, plan.dest_row))
+        check_same_device(rows, out, topk_weights, plan.dest_row)
         _lib.check(_lib.lib().dgb200_moe_unpermute(
             rows.data_ptr(), _stride(rows), topk_weights.data_ptr() if topk_weights is not None else None, plan.dest_row.data_ptr(),
             out.data_ptr(), _stride(out), tokens, topk, rows.size(1), rows.size(0), int(rows.dtype == torch.float32), _lib.current_stream_ptr()))
@@ -179,11 +191,10 @@ def moe_unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, plan: MoeDispat
     """Gradients of ``moe_unpermute``: ``(d_rows, d_weights)`` with ``d_rows[plan.dest_row[t, k]] = topk_weights[t, k] * dy[t]`` (padding
     rows of the segments zero, rows behind the last segment left as they are; written into ``out`` if given) and
     ``d_weights[t, k] = <rows[plan.dest_row[t, k]], dy[t]>``, float32, zero for masked entries."""
-    _check_plan(plan)
-    tokens, topk = plan.dest_row.shape
+    tokens, topk, experts, capacity = _check_plan(plan)
     _check_rows(rows, None, None, (torch.bfloat16, torch.float32), 'rows')
-    if rows.size(0) < plan.capacity:
-        raise RuntimeError(f'rows must hold plan.capacity ({plan.capacity}) rows, got {rows.size(0)}')
+    if rows.size(0) < capacity:
+        raise RuntimeError(f'rows must hold plan.capacity ({capacity}) rows, got {rows.size(0)}')
     _check_rows(dy, tokens, rows.size(1), (rows.dtype,), 'dy')
     _check_weights(topk_weights, plan)
     with _lib.on_device(rows.device):
@@ -197,5 +208,5 @@ def moe_unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, plan: MoeDispat
         _lib.check(_lib.lib().dgb200_moe_unpermute_backward(
             dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), topk_weights.data_ptr() if topk_weights is not None else None,
             plan.dest_row.data_ptr(), plan.expert_end.data_ptr(), out.data_ptr(), _stride(out), d_weights.data_ptr(), tokens, topk,
-            plan.num_experts, plan.alignment, rows.size(1), rows.size(0), int(rows.dtype == torch.float32), _lib.current_stream_ptr()))
+            experts, plan.alignment, rows.size(1), rows.size(0), int(rows.dtype == torch.float32), _lib.current_stream_ptr()))
     return out, d_weights
