@@ -476,6 +476,14 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
         while (ok && sched.next(t)) {
             if (t.group < 0) continue;
             const bool warp_has_rows = static_cast<int>(q * 32) < t.rows;
+            if constexpr (kF32) {
+                // c on its way into L2 while the tile is multiplied: all SMs ask for it at once at the end
+                if (p.c != nullptr && r < t.rows) {
+                    const int col = t.n0 + static_cast<int>(half) * kCols;
+                    const float* c = p.c + static_cast<long long>(t.row0 + r) * p.c_row_stride + col;
+                    for (int i = 0; i < kCols && col + i < p.n; i += 32) prefetch_l2(c + i);
+                }
+            }
             float acc[kCols];
 #pragma unroll
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;

@@ -82,17 +82,16 @@ int launch_block_scaled_split(const CUtensorMap& tm_a, const CUtensorMap& tm_b, 
     return 0;
 }
 
-// CTAs per tile of a dense GEMM (1: no split): the largest of 8, 4 and 2 for which all clusters run at once and every part keeps at least 8
-// (12 where more than 64 rows have to be added up) K blocks. Device time of calls back to back, no split (the narrowest tiles) -> split
-// (us): 7 x 4096 x 7168 15.7 -> 11.0 (4), 1 x 7168 x 2048 10.2 -> 7.8 (2), 33 x 1536 x 7168 15.1 -> 10.5 (4; 8: 11.1), 256 x 4096 x 7168 27.6 ->
-// 15.7 (2), 128 x 7168 x 16384 58.8 -> 29.4 (2). With less K it does not pay: 128 x 4096 x 2048 7.0 -> 9.6 (2), 11.7 (4); 128 x 4096 x
-// 1024 5.2 -> 8.5 (2).
-int block_scaled_split(long long tiles, int rows, int num_kb, bool f32, int sms, int* split) {
+// CTAs per tile of a dense GEMM (1: no split): the largest of 8, 4 and 2 for which all clusters run at once and every part keeps at least 12
+// K blocks. Device time of calls back to back, no split -> split (us): 7 x 4096 x 7168 15.7 -> 11.0 (4), 33 x 1536 x 7168 15.1 -> 10.5
+// (4; 8: 11.1), 512 x 2112 x 7168 16.3 -> 15.4 (2), 128 x 7168 x 16384 35.1 -> 29.4 (2). With less K it does not pay: 1 x 7168 x 2048 7.2 -> 7.8
+// (2), 64 x 7168 x 2048 7.5 -> 9.3 (2), 128 x 4096 x 2048 7.0 -> 9.6 (2).
+int block_scaled_split(long long tiles, int num_kb, bool f32, int sms, int* split) {
     *split = 1;
     if (tuning().split_k == 0) return 0;
     const int units = (num_kb + kScaleKb - 1) / kScaleKb;
     for (const int s : {8, 4, 2}) {
-        if (tuning().split_k > 0 ? s != tuning().split_k || units < s : units < (rows > 64 ? 3 : 2) * s) continue;
+        if (tuning().split_k > 0 ? s != tuning().split_k || units < s : units < 3 * s) continue;
         if (tiles * s > sms) continue;
         int clusters = 0;
         const CUtensorMap none{};
@@ -161,16 +160,25 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     const long long expected = masked ? std::min<long long>(std::max(a.expected_m, 1), a.m) : (psum ? (a.m + groups - 1) / groups : a.m);
     const long long m_tiles = groups * ((expected + 127) / 128);
     auto tiles_at = [&](int bn) { return m_tiles * ((a.n + bn - 1) / bn); };
+    // The tile width whose waves take the least time: a K block of a 256-, 128-, 64- or 32-wide tile takes about 540, 310, 260 or 240 ns, the
+    // narrow ones because a K block has fixed costs. 1999 x 2112 x 7168 (FP32, accumulated): 144 tiles of 256 52 us, 272 of 128 56.
     int block_n = 256;
     if (tuning().block_n != 0) {
         block_n = tuning().block_n;
     } else {
-        const int narrowest = a.b_mn_major ? 128 : 32;
-        while (block_n > narrowest && tiles_at(block_n) < sms) block_n /= 2;
+        long long best = -1;
+        constexpr int kWidths[4] = {256, 128, 64, 32}, kCost[4] = {54, 31, 26, 24};
+        for (int i = 0; i < (a.b_mn_major ? 2 : 4); ++i) {
+            const long long cost = (tiles_at(kWidths[i]) + sms - 1) / sms * kCost[i];
+            if (best < 0 || cost < best) {
+                best = cost;
+                block_n = kWidths[i];
+            }
+        }
     }
     int split = 1;
     if (dense && tuning().block_n == 0) {
-        if (const int rc = block_scaled_split(tiles_at(128), a.m, (a.k + 127) / 128, a.d_is_fp32 != 0, sms, &split)) return rc;
+        if (const int rc = block_scaled_split(tiles_at(128), (a.k + 127) / 128, a.d_is_fp32 != 0, sms, &split)) return rc;
         if (split > 1) block_n = 128;
     }
     // Pairs load 32 KB per SM and K block instead of 48. Single CTAs -> pairs (us): dense 4096 x 4096 x 7168 125 -> 117, 8192 x 7168 x 4096
@@ -308,14 +316,18 @@ int check_swiglu(const SwigluParams& p, bool backward, int out_width, int out_es
     return 0;
 }
 
-constexpr int kSwigluRows = 2;
+constexpr int kSwigluRows = 4;
 
-// A thread per vector of the row, in CTAs no wider than the row.
-void swiglu_launch_shape(int rows, long long vecs, dim3* grid, dim3* block) {
+// A thread per vector of the row, in CTAs no wider than the row. Returns the rows a thread takes: four, so that 8 (backward 12) loads are in
+// flight, where that leaves CTAs enough, else one. Backward 36864 x 2 x 2048 with its forward: one row a thread 211 us, two 195, four 181.
+int swiglu_launch_shape(int rows, long long vecs, int sms, dim3* grid, dim3* block) {
     const long long blocks = (vecs + 255) / 256;
     const long long threads = ((vecs + blocks - 1) / blocks + 31) / 32 * 32;
-    *grid = dim3(static_cast<unsigned>((rows + kSwigluRows - 1) / kSwigluRows), static_cast<unsigned>((vecs + threads - 1) / threads));
+    const long long columns = (vecs + threads - 1) / threads;
+    const int per_thread = (rows + kSwigluRows - 1) / kSwigluRows * columns * threads >= sms * 1024ll ? kSwigluRows : 1;
+    *grid = dim3(static_cast<unsigned>((rows + per_thread - 1) / per_thread), static_cast<unsigned>(columns));
     *block = dim3(static_cast<unsigned>(threads));
+    return per_thread;
 }
 
 int run_swiglu(const SwigluParams& p, bool backward, cudaStream_t stream) {
@@ -324,13 +336,15 @@ int run_swiglu(const SwigluParams& p, bool backward, cudaStream_t stream) {
     const bool wide = p.inter % 8 == 0 && p.x_stride % 8 == 0 && p.out_stride % 8 == 0 && (!backward || p.dy_stride % 8 == 0) &&
                       aligned_to(p.x, 16) && aligned_to(p.out, 16) && aligned_to(p.dy, 16);
     dim3 grid, block;
-    swiglu_launch_shape(p.rows, wide ? p.inter / 8 : p.inter, &grid, &block);
+    int sms = 0;
+    if (const int rc = effective_num_sms(&sms)) return rc;
+    const bool many = swiglu_launch_shape(p.rows, wide ? p.inter / 8 : p.inter, sms, &grid, &block) == kSwigluRows;
     DGB_REQUIRE(grid.y <= 65535u, "inter (%d) is too large", p.inter);
-    if (backward)
-        DGB_CUDA(launch_kernel(wide ? dgb200_swiglu_backward_kernel<8, kSwigluRows> : dgb200_swiglu_backward_kernel<1, kSwigluRows>, grid, block, 0,
-                               stream, use_pdl(), p));
-    else
-        DGB_CUDA(launch_kernel(wide ? dgb200_swiglu_kernel<8, kSwigluRows> : dgb200_swiglu_kernel<1, kSwigluRows>, grid, block, 0, stream, use_pdl(), p));
+    auto kernel = backward ? (wide ? (many ? dgb200_swiglu_backward_kernel<8, kSwigluRows> : dgb200_swiglu_backward_kernel<8, 1>)
+                                   : (many ? dgb200_swiglu_backward_kernel<1, kSwigluRows> : dgb200_swiglu_backward_kernel<1, 1>))
+                           : (wide ? (many ? dgb200_swiglu_kernel<8, kSwigluRows> : dgb200_swiglu_kernel<8, 1>)
+                                   : (many ? dgb200_swiglu_kernel<1, kSwigluRows> : dgb200_swiglu_kernel<1, 1>));
+    DGB_CUDA(launch_kernel(kernel, grid, block, 0, stream, use_pdl(), p));
     return 0;
 }
 
@@ -420,6 +434,13 @@ int dgb200_moe_dispatch_plan(const int64_t* topk_idx, int32_t num_tokens, int32_
     const int chunks = static_cast<int>((entries + chunk - 1) / chunk);
     DGB_REQUIRE(chunks <= 1 || (workspace != nullptr && aligned_to(workspace, 4)), "the plan needs its workspace");
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (entries <= kPlanThreads) {
+        const int threads = std::max<int>(32, (std::max<int>(static_cast<int>(entries), num_experts) + 31) / 32 * 32);
+        const size_t smem = static_cast<size_t>((entries + 31) / 32) * ((num_experts + 3) / 4 * 4);
+        DGB_CUDA(launch_kernel(dgb200_sort_small_kernel, dim3(1), dim3(threads), smem, stream, use_pdl(), reinterpret_cast<const long long*>(topk_idx),
+                               static_cast<int>(entries), num_experts, alignment, dest_row, expert_start, expert_end));
+        return 0;
+    }
     int* hist = chunks > 1 ? static_cast<int*>(workspace) : nullptr;
     const long long* idx = reinterpret_cast<const long long*>(topk_idx);
     if (hist != nullptr)
@@ -465,12 +486,13 @@ int dgb200_moe_permute(const void* x, int64_t x_row_bytes, int64_t x_row_stride_
     p.alignment = alignment;
     p.capacity = capacity;
     p.padding_blocks = zero_padding ? (alignment - 1 + 7) / 8 : 0;
-    const long long blocks = num_tokens + static_cast<long long>(num_experts) * p.padding_blocks;
-    DGB_REQUIRE(blocks < (1ll << 31), "too many rows");
-    if (blocks == 0 || capacity == 0) return 0;
+    if ((num_tokens == 0 && p.padding_blocks == 0) || capacity == 0) return 0;
     int sms = 0;
     if (const int rc = effective_num_sms(&sms)) return rc;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(column_blocks(num_tokens, p.rows.row_vecs, 256, sms)));
+    p.column_blocks = column_blocks(num_tokens, p.rows.row_vecs, 256, sms);
+    const long long ctas = static_cast<long long>(num_tokens) * p.column_blocks + static_cast<long long>(num_experts) * p.padding_blocks;
+    DGB_REQUIRE(ctas < (1ll << 31), "too many rows");
+    const dim3 grid(static_cast<unsigned>(ctas));
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     switch (vec_used) {
         case 16: return launch_permute<uint4, uint32_t>(p, grid, stream);
@@ -580,9 +602,11 @@ int dgb200_swiglu_per_token_cast_to_fp8(const void* x, int64_t x_row_stride, voi
     DGB_REQUIRE((sf != nullptr || rows == 0) && aligned_to(sf, 4) && sf_row_stride >= (inter + 127) / 128, "scale rows must hold one scale per 128 values");
     if (rows == 0) return 0;
     dim3 grid, block;
-    swiglu_launch_shape(rows, (inter + 127) / 128 * 16, &grid, &block);
+    int sms = 0;
+    if (const int rc = effective_num_sms(&sms)) return rc;
+    const bool many = swiglu_launch_shape(rows, (inter + 127) / 128 * 16, sms, &grid, &block) == kSwigluRows;
     DGB_REQUIRE(grid.y <= 65535u, "inter (%d) is too large", inter);
-    DGB_CUDA(launch_kernel(dgb200_swiglu_cast_kernel<kSwigluRows>, grid, block, 0, static_cast<cudaStream_t>(stream), use_pdl(), p));
+    DGB_CUDA(launch_kernel(many ? dgb200_swiglu_cast_kernel<kSwigluRows> : dgb200_swiglu_cast_kernel<1>, grid, block, 0, static_cast<cudaStream_t>(stream), use_pdl(), p));
     return 0;
 }
 

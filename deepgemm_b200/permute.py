@@ -107,9 +107,9 @@ def moe_dispatch_plan(topk_idx: torch.Tensor, num_experts: int, alignment: Optio
     lib = _lib.lib()
     workspace_bytes = lib.dgb200_moe_dispatch_plan_workspace_bytes(tokens, topk, num_experts)
     with _lib.on_device(topk_idx.device):
-        dest = torch.empty((tokens, topk), dtype=torch.int32, device=topk_idx.device)
-        start, end = torch.empty((2, num_experts), dtype=torch.int32, device=topk_idx.device).unbind(0)
-        workspace = torch.empty(workspace_bytes, dtype=torch.int8, device=topk_idx.device) if workspace_bytes else None
+        dest = topk_idx.new_empty((tokens, topk), dtype=torch.int32)
+        start, end = topk_idx.new_empty((2, num_experts), dtype=torch.int32).unbind(0)
+        workspace = topk_idx.new_empty(workspace_bytes, dtype=torch.int8) if workspace_bytes else None
         _lib.check(lib.dgb200_moe_dispatch_plan(
             topk_idx.data_ptr(), tokens, topk, num_experts, alignment, dest.data_ptr(), start.data_ptr(), end.data_ptr(),
             workspace.data_ptr() if workspace is not None else None, _lib.current_stream_ptr()))
