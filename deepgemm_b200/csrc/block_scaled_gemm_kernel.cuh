@@ -487,7 +487,8 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             float acc[kCols];
 #pragma unroll
             for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
-#pragma unroll 1
+// twice: the jump back costs an instruction fetch (8192 x 7168 x 4096 on pairs 226 -> 216 us)
+#pragma unroll 2
             for (int kb = first_kb; kb < num_kb; ++kb) {
                 const uint32_t as = it % kAccums;
                 ok = mbar_wait(tmem_full_bar + as, (it / kAccums) & 1, abort_flag, kTimeoutTmemFull, kb);

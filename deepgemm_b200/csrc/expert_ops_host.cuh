@@ -181,8 +181,8 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
         if (const int rc = block_scaled_split(tiles_at(128), (a.k + 127) / 128, a.d_is_fp32 != 0, sms, &split)) return rc;
         if (split > 1) block_n = 128;
     }
-    // Pairs load 32 KB per SM and K block instead of 48. Single CTAs -> pairs (us): dense 4096 x 4096 x 7168 125 -> 117, 8192 x 7168 x 4096
-    // 255 -> 226. With groups half a pair tile is lost on every second one: N 4096, K 7168, 32 groups of 247 rows 323 -> 371, 8 of
+    // Pairs load 32 KB per SM and K block instead of 48. Single CTAs -> pairs (us): dense 4096 x 4096 x 7168 116 -> 111, 8192 x 7168 x 4096
+    // 228 -> 216. With groups half a pair tile is lost on every second one: N 4096, K 7168, 32 groups of 247 rows 323 -> 371, 8 of
     // 900 239 -> 250, 4 of 2000 248 -> 250.
     const long long pair_tiles = groups * ((expected + 255) / 256) * ((a.n + 255) / 256);
     const bool pair = !row_ids && block_n == 256 && sms >= 2 && tuning().pair != 0 &&
