@@ -91,15 +91,15 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
         raise RuntimeError(f'd must be a CUDA tensor of shape {shape} with unit stride on N, {" or ".join(map(str, kinds))}')
     if masked and not d.is_contiguous():
         raise RuntimeError('d must be contiguous')
-    row_stride = d.stride(-2) if m > 1 else max(d.stride(-2), n)
+    row_stride = d.stride(-2) if m > 1 else n
     if row_stride < n or row_stride * d.element_size() % 16 != 0:
         raise RuntimeError('d rows must be 16-byte aligned and not overlap')
     if c is not None:
         if not (c.is_cuda and c.dtype == torch.float32 and d.dtype == torch.float32 and c.shape == d.shape):
             raise RuntimeError('c must be a CUDA float32 tensor of the shape of a float32 d')
         same = c.data_ptr() == d.data_ptr() and c.stride() == d.stride()
-        if not same and (overlap(c, d) or c.stride(-1) != 1 or c.stride(-2) % 4 != 0 or c.stride(-2) < n or c.data_ptr() % 16 != 0):
-            c = c.contiguous() if not overlap(c, d) else c.clone(memory_format=torch.contiguous_format)
+        if not same and (overlap(c, d) or c.stride(-1) != 1 or (m > 1 and (c.stride(-2) % 4 != 0 or c.stride(-2) < n)) or c.data_ptr() % 16 != 0):
+            c = c.clone(memory_format=torch.contiguous_format)
     check_same_device(a_q, a_sf, b_q, b_sf, d, c, layout)
     if m == 0:
         return
@@ -112,7 +112,7 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
         _ARGS.size, a_q.data_ptr(), a_sf.data_ptr(), b_q.data_ptr(), b_sf.data_ptr(), d.data_ptr(), c.data_ptr() if c is not None else 0,
         layout.data_ptr() if layout is not None else 0, a_sf.stride(0) if masked else 0, a_sf.stride(-2), a_sf.stride(-1),
         0 if dense else b_sf.stride(0), b_sf.stride(-2), b_sf.stride(-1), row_stride,
-        (c.stride(-2) if m > 1 else max(c.stride(-2), n)) if c is not None else 0, m, n, k, groups, layout_kind, alignment,
+        (c.stride(-2) if m > 1 else n) if c is not None else 0, m, n, k, groups, layout_kind, alignment,
         int(bool(store_padding)), int(expected_m), int(b_mn_major), int(d.dtype == torch.float32))
     with _lib.on_device(d.device):
         _lib.check(_lib.lib().dgb200_fp8_block_scaled_gemm(args, _lib.current_stream_ptr()))

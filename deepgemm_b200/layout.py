@@ -86,7 +86,8 @@ def transform_sf_into_required_layout(sf: torch.Tensor, mn: int, k: int,
     check_sf_layout(sf, mn, k, gran_mn, gran_k, num_groups)
     if sf.dtype == torch.float32 and gran_k in (32, 128):
         if disable_ue8m0_cast:
-            raise RuntimeError('disable_ue8m0_cast: nothing to transform, the GEMMs take such scales as they are')
+            raise RuntimeError('disable_ue8m0_cast: the FP8 GEMMs take float32 scales as they are where both operands have them, '
+                               'there is no layout to transform them into')
         if gran_mn != 1:
             index = torch.arange(mn, device=sf.device) // gran_mn
             sf = sf.index_select(-2, index)

@@ -41,7 +41,8 @@ int dgb200_get_num_sms(void);
 
 /* Process-wide tuning knobs of the GEMM kernels. Plays the role of the reference's heuristics overrides
  * (csrc/apis/runtime.hpp:21-41).
- *   "block_n"            0 = automatic, 128 or 256: width of an output tile of the tokens-on-M kernel.
+ *   "block_n"            0 = automatic, 128 or 256: width of an output tile of the tokens-on-M kernel and of the FP8 GEMM with FP32 scales
+ *                        (which also has 64 and 32, and with a width given does not split K).
  *   "swap_ab"            layer GEMMs: -1 = choose the tile orientation from the expected rows per expert (default:
  *                        swapped-operand kernel alone for decode-sized batches, experts split by size around 128
  *                        rows per expert, tokens-on-M kernel otherwise), 0 = tokens-on-M kernel only, 1 = everything
@@ -50,7 +51,8 @@ int dgb200_get_num_sms(void);
  *   "split_k"            dense GEMMs: -1 (default) = K split over 2, 4 or 8 CTAs where few tiles have a long K, 0 = never (a row's
  *                        bits then do not depend on the batch it is in), 2 / 4 / 8 = that split wherever the form exists.
  *   "pair"               GEMMs on CTA pairs (256 x 256 tiles): -1 (default) = by size, 0 = never, 1 = wherever the form exists
- *                        (BF16; FP8 and NVFP4 layers, whose scale factors lie in tcgen05.cp order; K-grouped). Same bits.
+ *                        (BF16; FP8 and NVFP4 layers, whose scale factors lie in tcgen05.cp order; K-grouped; FP8 with FP32
+ *                        scales). Same bits.
  *   "fused_dispatch"     expert-parallel layer with guest experts: 0 (default) = the dispatch push is a kernel of its own;
  *                        1 or a phase count 2..4 = several expert phases, and the epilogue warps of the gate/up GEMM of
  *                        phase q also push the rows this rank routes to phase q + 1 (measured slower than the default:

@@ -24,7 +24,7 @@ def tuning():
     def set_knob(name, value):
         _lib.check(_lib.lib().dgb200_set_tuning(name.encode(), value))
     yield set_knob
-    for name, value in (('block_n', 0), ('pair', -1)):
+    for name, value in (('block_n', 0), ('pair', -1), ('split_k', -1)):
         set_knob(name, value)
 
 
@@ -90,6 +90,72 @@ def test_dense_every_tile_form(dg, tuning, block_n, pair, m, n, k, mn_major):
         d = torch.full((m, n), float('nan'), dtype=dtype, device='cuda')
         dg.fp8_gemm_nt(a, used, d, disable_ue8m0_cast=True)
         check(d, want, s, k)
+
+
+@pytest.mark.parametrize('split', [2, 4, 8])
+@pytest.mark.parametrize('m, n, k', [(1, 8, 4112), (7, 264, 4096), (64, 520, 7168), (130, 392, 8176), (300, 128, 5120)])
+@pytest.mark.parametrize('mn_major', [False, True])
+def test_split_k(dg, tuning, split, m, n, k, mn_major):
+    """K split over a cluster: one more FP32 addition per part, which the tolerance's K blocks cover. The same bits in every run."""
+    if mn_major and n % 16 != 0:
+        n += 8
+    tuning('split_k', split)
+    a, b = operand(m, k, seed=61, block_rows=1), operand(n, k, seed=62, block_rows=128)
+    used = (b[0].t().contiguous().t(), b[1]) if mn_major else b
+    want, s = reference(a, b)
+    c = torch.randn(m, n, device='cuda')
+    for dtype, acc in ((torch.bfloat16, None), (torch.float32, None), (torch.float32, c)):
+        outs = []
+        for _ in range(2):
+            store = torch.full((m + 1, n + 16), float('nan'), dtype=dtype, device='cuda')
+            dg.fp8_gemm_nt(a, used, store[:m, :n], c=acc, disable_ue8m0_cast=True)
+            outs.append(store[:m, :n].clone())
+            assert torch.isnan(store[m].float()).all() and torch.isnan(store[:, n:].float()).all()
+        check(outs[0], want + (c.double() if acc is not None else 0), s, k, extra=0 if acc is None else c.double().abs() + want.abs())
+        assert torch.equal(outs[0], outs[1])
+
+
+def test_a_long_k_is_split_by_itself_and_only_where_allowed(dg, tuning):
+    m, n, k = 5, 512, 7168
+    a, b = operand(m, k, seed=63, block_rows=1), operand(n, k, seed=64, block_rows=128)
+    want, s = reference(a, b)
+    outs = []
+    for split in (-1, 0):
+        tuning('split_k', split)
+        d = torch.empty((m, n), device='cuda')
+        dg.fp8_gemm_nt(a, b, d, disable_ue8m0_cast=True)
+        check(d, want, s, k)
+        outs.append(d)
+    assert not torch.equal(*outs)  # another order of the sum
+
+
+def test_every_tile_form_gives_the_same_bits(dg, tuning):
+    m, n, k = 600, 1040, 1168
+    a, b = operand(m, k, seed=65, block_rows=1), operand(n, k, seed=66, block_rows=128)
+    outs = []
+    for block_n, pair in ((0, -1), (128, 0), (256, 0), (256, 1)):
+        tuning('block_n', block_n)
+        tuning('pair', pair)
+        d = torch.empty((m, n), device='cuda')
+        dg.fp8_gemm_nt(a, b, d, disable_ue8m0_cast=True)
+        outs.append(d)
+    # narrow tiles are for few of them: the same rows in a batch of their own
+    small = torch.empty((3, n), device='cuda')
+    tuning('block_n', 0)
+    tuning('pair', -1)
+    dg.fp8_gemm_nt((a[0][:3], a[1][:3]), b, small, disable_ue8m0_cast=True)
+    assert all(torch.equal(o, outs[0]) for o in outs) and torch.equal(small, outs[0][:3])
+
+
+def test_accumulator_of_any_layout(dg):
+    m, n, k = 40, 72, 272
+    a, b = operand(m, k, seed=67, block_rows=1), operand(n, k, seed=68, block_rows=128)
+    want, s = reference(a, b)
+    wide_c = torch.randn(m + 1, 2 * n + 1, device='cuda')
+    for c in (wide_c[:m, 1:n + 1], wide_c[1:, ::2][:, :n], wide_c[:1, :n].expand(m, n), wide_c.t()[:n, :m].t()):
+        d = torch.empty((m, n), device='cuda')
+        dg.fp8_gemm_nt(a, b, d, c=c, disable_ue8m0_cast=True)
+        check(d, want + c.double(), s, k, extra=c.double().abs() + want.abs())
 
 
 @pytest.mark.parametrize('where', ['apart', 'in place', 'strided', 'overlapping'])
