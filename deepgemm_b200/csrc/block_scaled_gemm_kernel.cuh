@@ -31,7 +31,7 @@ struct BlockScaledParams {
     int m, n, k, num_groups, alignment, store_padding;
     int b_mn_major;   // B is [groups, k, n] with n contiguous
     int sf_vec;       // the scales of four consecutive K blocks lie in 16 aligned bytes, for a as for b
-    int a_box_rows;   // rows of A that one load brings: 128, or fewer where no tile has more
+    int a_box_rows;   // rows of A that one load brings: 128, or fewer where tiles have few (a tile takes as many loads as its rows need)
 };
 
 // kind::f8f6f4 descriptor: E4M3 operands (format 0), FP32 accumulator.
@@ -339,13 +339,16 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             bool ok = true;
             while (ok && sched.next(t)) {
                 if (t.group < 0) continue;
+                const int a_loads = kPair ? 1 : (t.rows + p.a_box_rows - 1) / p.a_box_rows;
                 for (int kb = first_kb; kb < num_kb; ++kb) {
                     ok = mbar_wait(empty_bar + stage, phase ^ 1, abort_flag, kTimeoutEmpty, kb);
                     if (!ok) break;
                     if (elected) {
                         if (is_a) {
-                            stage_arrive(stage, static_cast<uint32_t>(p.a_box_rows) * 128);
-                            load_tile(L::kOffA + stage * L::kABytes, &tm_a, stage, kb * 128, t.row0, p.mode == kModeMasked ? t.group : 0);
+                            stage_arrive(stage, static_cast<uint32_t>(a_loads * p.a_box_rows) * 128);
+                            for (int i = 0; i < a_loads; ++i)
+                                load_tile(L::kOffA + stage * L::kABytes + i * p.a_box_rows * 128, &tm_a, stage, kb * 128, t.row0 + i * p.a_box_rows,
+                                          p.mode == kModeMasked ? t.group : 0);
                         } else {
                             stage_arrive(stage, L::kBBytes);
                             const int off = L::kOffB + stage * L::kBBytes;

@@ -162,13 +162,16 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     auto tiles_at = [&](int bn) { return m_tiles * ((a.n + bn - 1) / bn); };
     // The tile width whose waves take the least time: a K block of a 256-, 128-, 64- or 32-wide tile takes about 540, 310, 260 or 240 ns, the
     // narrow ones because a K block has fixed costs. 1999 x 2112 x 7168 (FP32, accumulated): 144 tiles of 256 52 us, 272 of 128 56.
+    // Groups of few rows read their weights at HBM rate, and tiles of 128 leave a shorter last wave: 32 groups of 24 rows, 256 -> 128 wide:
+    // N 7168, K 2048 89 -> 84 us, N 4096, K 7168 161 -> 154; 64 of 8 rows, N 4096, K 4096 169 -> 171.
+    const bool few_rows = (masked || psum) && expected <= 96;
     int block_n = 256;
     if (tuning().block_n != 0) {
         block_n = tuning().block_n;
     } else {
         long long best = -1;
         constexpr int kWidths[4] = {256, 128, 64, 32}, kCost[4] = {54, 31, 26, 24};
-        for (int i = 0; i < (a.b_mn_major ? 2 : 4); ++i) {
+        for (int i = few_rows ? 1 : 0; i < (a.b_mn_major ? 2 : 4); ++i) {
             const long long cost = (tiles_at(kWidths[i]) + sms - 1) / sms * kCost[i];
             if (best < 0 || cost < best) {
                 best = cost;
@@ -189,6 +192,9 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
                       (tuning().pair == 1 || (expected > (dense ? 128 : 2048) && pair_tiles * 2 >= sms));
     p.a_box_rows = 128;
     if (!pair && (dense || masked) && a.m < 128) p.a_box_rows = (a.m + 7) / 8 * 8;
+    // Groups of few rows: 32 at a time, as many as the tile has; a 128-row load would bring the other rows of the buffer as well
+    // (32 groups of 24 rows, N 4096, K 7168: 163 -> 154 us; 64 of 8, N 4096, K 4096: 176 -> 169).
+    if (!pair && few_rows) p.a_box_rows = std::min(p.a_box_rows, 32);
 
     CUtensorMap tm_a, tm_b;
     int rc = make_tensor_map_3d_bytes(&tm_a, a.a, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.m), masked ? a.num_groups : 1,
