@@ -389,8 +389,9 @@ int dgb200_per_token_cast_to_fp8_f32_scales(const void* x, int64_t x_row_stride,
     // four rows a warp keep 64 bytes a lane in flight; where that would leave SMs without a CTA, one row
     const bool few = static_cast<long long>((rows + 31) / 32) * columns < 2 * sms;
     const dim3 grid(static_cast<unsigned>(few ? (rows + 7) / 8 : (rows + 31) / 32), columns);
-    DGB_CUDA(launch_kernel(few ? dgb200_cast_rows_f32_kernel<1> : dgb200_cast_rows_f32_kernel<4>, grid, dim3(256), 0,
-                           static_cast<cudaStream_t>(stream_), use_pdl(), p));
+    auto kernel = few ? dgb200_cast_rows_f32_kernel<1, false>
+                      : (gran_k == 128 ? dgb200_cast_rows_f32_kernel<4, true> : dgb200_cast_rows_f32_kernel<4, false>);
+    DGB_CUDA(launch_kernel(kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream_), use_pdl(), p));
     return 0;
 }
 

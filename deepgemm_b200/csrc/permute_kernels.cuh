@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(128) dgb200_unpermute_kernel(const UnpermutePa
 // masked entry); padding rows of d_rows = 0, as the K-grouped GEMM wants them, rows behind the last segment stay. One CTA per token: dy is
 // read once and kept, the dot products are summed in a fixed order (thread, warp, CTA).
 template <typename T, int kVec>
-__global__ void __launch_bounds__(256) dgb200_unpermute_backward_kernel(const UnpermuteParams p) {
+__global__ void __launch_bounds__(256, 4) dgb200_unpermute_backward_kernel(const UnpermuteParams p) {
     using V = RowVec<T, kVec>;
     using Raw = typename V::Raw;
     pdl_prologue();

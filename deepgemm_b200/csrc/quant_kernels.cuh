@@ -342,24 +342,35 @@ __global__ void __launch_bounds__(256) dgb200_cast_rows_nvfp4_kernel(const CastN
 // NaN stays NaN and is passed over by the maximum; a block that holds an infinity has the scale infinity, its infinities become
 // NaN and the rest zero, as the division gives.
 // ------------------------------------------------------------------------------------------------------------------
+// The quotients are formed with the sign turned, two at a time, and turned back in the codes: with y' = -1/sf the steps are q' = v y',
+// r = v + q' sf, q' + r y', and a zero comes out with v's sign (the other way round a residual of +0 would make +0 of -0).
+__device__ __forceinline__ void negated_quotients(float v0, float v1, float sf, float minus_y, float& q0, float& q1) {
+    asm("{\n\t"
+        ".reg .b64 v, y, s, q, r;\n\t"
+        "mov.b64 v, {%2, %3};\n\t"
+        "mov.b64 y, {%4, %4};\n\t"
+        "mov.b64 s, {%5, %5};\n\t"
+        "mul.rn.f32x2 q, v, y;\n\t"
+        "fma.rn.f32x2 r, q, s, v;\n\t"
+        "fma.rn.f32x2 q, r, y, q;\n\t"
+        "mov.b64 {%0, %1}, q;\n\t"
+        "}\n" : "=f"(q0), "=f"(q1) : "f"(v0), "f"(v1), "f"(minus_y), "f"(sf));
+}
+
 __device__ __forceinline__ uint4 e4m3_quotients(const float* v, float sf, float y, bool special) {
     float q[16];
     if (special) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = v[i] / sf;
+        for (int i = 0; i < 16; ++i) q[i] = v[i] / -sf;
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float q0 = v[i] * y;
-            // the residual step turns -0 into 0: the sign is v's in every case
-            q[i] = __uint_as_float(__float_as_uint(fmaf(fmaf(-q0, sf, v[i]), y, q0)) | (__float_as_uint(v[i]) & 0x80000000u));
-        }
+        for (int i = 0; i < 16; i += 2) negated_quotients(v[i], v[i + 1], sf, -y, q[i], q[i + 1]);
     }
     uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const __nv_fp8x4_e4m3 q4(make_float4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]));
-        o[i] = q4.__x;
+        o[i] = q4.__x ^ 0x80808080u;
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
@@ -374,14 +385,17 @@ struct CastF32Params {
     int rows, k, gran_k, ue8m0;
 };
 
-// One scale per row and gran_k (32 or 128) columns. A lane owns 16 consecutive columns of kRows rows; a warp spans 512 columns.
-template <int kRows>
+// One scale per row and gran_k (32 or 128) columns. A lane owns 16 consecutive columns of kRows rows; a warp spans 512 columns. The arithmetic
+// bounds it, not HBM: 8192 x 7168 took 41.8 us when every lane divided for each of its four rows; with the rows' two divisions shared
+// out among the lanes of a block (kShared: gran_k = 128, four rows) and the quotients formed two at a time 32.7, at the copy rate 27.
+template <int kRows, bool kShared>
 __global__ void __launch_bounds__(256) dgb200_cast_rows_f32_kernel(const CastF32Params p) {
+    static_assert(!kShared || kRows == 4, "lane l of a block divides for row l % 4");
     pdl_prologue();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.y * 512 + lane * 16;
     const long long row0 = (blockIdx.x * 8ll + warp) * kRows;
-    const int lanes_per_block = p.gran_k / 16;
+    const int lanes_per_block = kShared ? 8 : p.gran_k / 16;
     const bool inside = col < p.k;  // k % 16 == 0
     uint4 raw[kRows][2];
 #pragma unroll
@@ -393,25 +407,50 @@ __global__ void __launch_bounds__(256) dgb200_cast_rows_f32_kernel(const CastF32
             raw[r][1] = ld_global_nc_v4(src + 1);
         }
     }
+    float amax[kRows];
+    bool special[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const uint32_t w[8] = {raw[r][0].x, raw[r][0].y, raw[r][0].z, raw[r][0].w, raw[r][1].x, raw[r][1].y, raw[r][1].z, raw[r][1].w};
+        amax[r] = amax_bf16x16(w, special[r]);
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1)
+            if (off < lanes_per_block) amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], off));
+        special[r] |= amax[r] == INFINITY;
+    }
+    float my_sf = 0.0f, my_y = 0.0f;
+    if constexpr (kShared) {
+        const int mine = lane & 3;
+        const float a = mine == 0 ? amax[0] : (mine == 1 ? amax[1 % kRows] : (mine == 2 ? amax[2 % kRows] : amax[3 % kRows]));
+        my_sf = fmaxf(a, 1e-4f) / 448.0f;
+        my_y = 1.0f / my_sf;
+        // (of a short last block the storing lane itself may lie outside)
+        if ((lane & 4) == 0 && blockIdx.y * 512 + (lane & 24) * 16 < p.k && row0 + mine < p.rows)
+            p.sf[(row0 + mine) * p.sf_row_stride + col / 128] = my_sf;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        float sf, y;
+        if constexpr (kShared) {
+            sf = __shfl_sync(0xffffffffu, my_sf, (lane & 24) | r);
+            y = __shfl_sync(0xffffffffu, my_y, (lane & 24) | r);
+        } else {
+            sf = fmaxf(amax[r], 1e-4f) / 448.0f;
+            y = 1.0f / sf;
+        }
+        if (!inside || row0 + r >= p.rows) continue;
+        const uint32_t w[8] = {raw[r][0].x, raw[r][0].y, raw[r][0].z, raw[r][0].w, raw[r][1].x, raw[r][1].y, raw[r][1].z, raw[r][1].w};
         float v[16];
         unpack_bf16x16(w, v);
-        bool special;
-        float amax = amax_bf16x16(w, special);
-        for (int off = 1; off < lanes_per_block; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-        if (!inside || row0 + r >= p.rows) continue;
-        const float sf = fmaxf(amax, 1e-4f) / 448.0f;
-        const uint4 q = e4m3_quotients(v, sf, 1.0f / sf, special || amax == INFINITY);
+        const uint4 q = e4m3_quotients(v, sf, y, special[r]);
         st_global_v4(p.q + (row0 + r) * p.q_row_stride + col, q.x, q.y, q.z, q.w);
-        if (lane % lanes_per_block == 0) p.sf[(row0 + r) * p.sf_row_stride + col / p.gran_k] = sf;
+        if (!kShared && lane % lanes_per_block == 0) p.sf[(row0 + r) * p.sf_row_stride + col / p.gran_k] = sf;
     }
 }
 
 // One scale per 128 x 128 block (a power of two with ue8m0 != 0: the smallest one not below amax / 448). One CTA per block keeps its 32 KB in
 // registers between the maximum and the quotients: 8 lanes hold a row's 128 columns, 32 rows at a time.
-__global__ void __launch_bounds__(256) dgb200_cast_blocks_f32_kernel(const CastF32Params p) {
+__global__ void __launch_bounds__(256, 4) dgb200_cast_blocks_f32_kernel(const CastF32Params p) {
     pdl_prologue();
     __shared__ float warp_amax[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

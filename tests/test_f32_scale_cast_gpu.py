@@ -48,6 +48,15 @@ def test_per_token(dg, rows, k, gran_k, scale):
     assert torch.equal(sf.cpu(), want_sf[:, 0]) and same(q, want_q[:, 0])
 
 
+@pytest.mark.parametrize('rows, k', [(20001, 528), (9999, 1040), (20000, 16), (5003, 2032)])
+@pytest.mark.parametrize('gran_k', [32, 128])
+def test_per_token_many_rows_with_a_short_last_block(dg, rows, k, gran_k):
+    x = values(rows, k, seed=4)
+    q, sf = dg.utils.per_token_cast_to_fp8(x.cuda(), use_ue8m0=False, gran_k=gran_k)
+    want_q, want_sf = reference(x[:, None], 1, gran_k)
+    assert torch.equal(sf.cpu(), want_sf[:, 0]) and same(q, want_q[:, 0])
+
+
 @pytest.mark.parametrize('shape', [(1, 16), (128, 128), (130, 272), (7, 1024), (513, 144), (3, 256, 128), (2, 200, 400), (5, 1, 16)])
 @pytest.mark.parametrize('ue8m0', [False, True])
 @pytest.mark.parametrize('scale', [1.0, 1e-30])
