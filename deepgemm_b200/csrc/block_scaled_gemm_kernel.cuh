@@ -6,9 +6,18 @@
 // the product of the two scales. Behavioural counterpart in the reference: its FP32-scale kernel of the previous architecture
 // (deep_gemm/include/deep_gemm/impls/sm90_fp8_gemm_1d2d.cuh), reached there with disable_ue8m0_cast.
 //
-// Warp roles (384 threads): warp 0 loads A tiles, warp 3 B tiles, warp 1 issues the MMAs, warp 2 owns the tensor memory,
+// Warp roles (384 threads): warp 0 loads A tiles, warp 3 B tiles, warp 1 issues the MMAs, warp 2 owns the tensor memory and brings the scales,
 // warps 4-11 add up (TMEM lane quarter = warp index % 4, two warps per quarter split the columns). A thread owns one row's
 // half of the tile in registers, so a scale is one scalar per thread and K block and no value crosses lanes until the store.
+//
+// What bounds it: the sums. A K block of a 128 x 256 tile is 512 cycles of MMAs, and each scheduler has two warps that read 128 columns of
+// tensor memory (60 cycles per 32 columns) and issue 64 packed multiply-adds (2.2 cycles each) for it, which take turns
+// rather than overlap, plus what the hand-over costs. Measured on the way, 4096 x 4096 x 7168 on pairs: scales read by the summing warps
+// 151 us; through a warp of their own, the MMA issuer's loop cut to one wait 124; fewer commits and counters 119; whole lines
+// stored 116; the loop unrolled twice 111 (2170 TFLOP/s; 8192 x 7168 x 4096 216 us, 2230). The power-of-two kernel, whose
+// scales the tensor core applies, takes 98: the power limit is then what stops it. Without the multiply-adds this one takes 97, with
+// half of them 103. What did not help: 16 summing warps (contention for the same ports: 134), 32-column loads (registers spill), one lane
+// polling for its warp (the divergence costs more), the halves of a tile on barriers of their own (no difference).
 #pragma once
 
 #include <cuda_bf16.h>
