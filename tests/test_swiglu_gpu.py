@@ -152,3 +152,19 @@ def test_graph_and_side_stream(dg):
     torch.cuda.synchronize()
     for a, b, c in zip(got, want, beside):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) and torch.equal(c.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize('rows, inter', [(3, 520), (300, 2048)])
+def test_fp8_arithmetic_is_that_of_fp32_operations(dg, rows, inter):
+    """The scales and codes are those of the formula in single FP32 operations. The kernel's reciprocal comes from one Newton step on one
+    that is at most 2^-22 off: 2^-44 and a rounding, another value than the division's for one in 2^20 (none or one of the values here). That
+    reaches one scale, and the codes of its block only where a quotient lies at a tie."""
+    x, _ = case(rows, inter, 0, seed=9)
+    gate, up = x[:, :inter].float(), x[:, inter:].float()
+    y = gate * (1.0 / (1.0 + torch.exp(-gate))) * up
+    blocks = -(-inter // 128)
+    amax = torch.nn.functional.pad(y, (0, blocks * 128 - inter)).view(rows, blocks, 128).abs().amax(dim=-1)
+    scale = amax.clamp(min=1e-4) / torch.full_like(amax, 448.0)
+    codes = (y / scale.repeat_interleave(128, dim=1)[:, :inter]).to(torch.float8_e4m3fn)
+    q, sf = dg.swiglu_per_token_cast_to_fp8(x)
+    assert (sf != scale).sum() <= 1 and (q.view(torch.uint8) != codes.view(torch.uint8)).sum() <= 1
