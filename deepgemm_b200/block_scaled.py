@@ -79,6 +79,8 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
         raise RuntimeError(f'K mismatch: a has {k}, b has {k_b}')
     if masked and a_q.size(0) != groups:
         raise RuntimeError(f'group count mismatch: a has {a_q.size(0)}, b has {groups}')
+    if max(m, n, k, groups) >= 2 ** 31:
+        raise RuntimeError('the operands are too large')
     if n % 8 != 0 or k % 16 != 0 or n == 0 or k == 0:
         raise RuntimeError(f'n ({n}) must be a positive multiple of 8 and k ({k}) of 16')
     if b_mn_major and n % 16 != 0:
@@ -104,7 +106,7 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
     if m == 0:
         return
     d0, d1 = span(d)
-    for t in (a_q, a_sf, b_q, b_sf):
+    for t in (a_q, a_sf, b_q, b_sf) if layout is None else (a_q, a_sf, b_q, b_sf, layout):
         t0, t1 = span(t)
         if t0 < d1 and d0 < t1:
             raise RuntimeError('d must not overlap an operand')

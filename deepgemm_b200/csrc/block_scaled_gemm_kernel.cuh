@@ -39,7 +39,7 @@ struct BlockScaledParams {
     int mode;  // kModeDense / kModeRowIds / kModePsum / kModeMasked (A and D [G, m, *])
     int m, n, k, num_groups, alignment, store_padding;
     int b_mn_major;   // B is [groups, k, n] with n contiguous
-    int sf_vec;       // the scales of four consecutive K blocks lie in 16 aligned bytes, for a as for b
+    int sf_vec;       // a row's scales of four consecutive K blocks lie in 16 aligned bytes
     int a_box_rows;   // rows of A that one load brings: 128, or fewer where tiles have few (a tile takes as many loads as its rows need)
 };
 

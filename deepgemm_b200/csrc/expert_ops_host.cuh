@@ -6,6 +6,9 @@
 namespace dgb {
 namespace {
 
+// Rows and columns a call may have: tiles and vectors are counted in 32 bits, with room for the last one.
+constexpr int kMaxRows = 0x7ffff000, kMaxColumns = 1 << 28;
+
 inline bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
 
 // Raises a kernel's shared-memory limit once per device.
@@ -110,6 +113,7 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     const bool row_ids = a.layout_kind == DGB200_LAYOUT_ROW_IDS, psum = a.layout_kind == DGB200_LAYOUT_PSUM;
     DGB_REQUIRE(dense || masked || row_ids || psum, "unknown layout kind %d", a.layout_kind);
     DGB_REQUIRE(a.m >= 0 && a.n > 0 && a.k > 0 && a.num_groups > 0, "m must be >= 0, n, k and num_groups positive");
+    DGB_REQUIRE(a.m <= kMaxRows && a.n <= kMaxColumns && a.k <= kMaxColumns, "m (%d), n (%d) or k (%d) is too large", a.m, a.n, a.k);
     DGB_REQUIRE(a.n % 8 == 0 && a.k % 16 == 0, "n (%d) must be a multiple of 8 and k (%d) of 16", a.n, a.k);
     DGB_REQUIRE(!a.b_mn_major || a.n % 16 == 0, "an MN-major b needs n (%d) to be a multiple of 16", a.n);
     DGB_REQUIRE(!dense || a.num_groups == 1, "the dense form has one group");
@@ -150,8 +154,7 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     p.alignment = dense || masked ? 128 : a.alignment;
     p.store_padding = a.store_padding;
     p.b_mn_major = a.b_mn_major ? 1 : 0;
-    p.sf_vec = a.sfa_k_stride == 1 && a.sfb_k_stride == 1 && aligned_to(a.sfa, 16) && aligned_to(a.sfb, 16) && a.sfa_row_stride % 4 == 0 &&
-               a.sfb_n_stride % 4 == 0 && a.sfa_group_stride % 4 == 0 && a.sfb_group_stride % 4 == 0;
+    p.sf_vec = a.sfa_k_stride == 1 && aligned_to(a.sfa, 16) && a.sfa_row_stride % 4 == 0 && a.sfa_group_stride % 4 == 0;
     int sms = 0;
     if (const int rc = effective_num_sms(&sms)) return rc;
 
@@ -231,6 +234,7 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
 
 int check_cast_f32(const void* x, const void* q, const float* sf, int rows, int k, long long x_row_stride, long long q_row_stride) {
     DGB_REQUIRE(rows >= 0 && k > 0 && k % 16 == 0, "k (%d) must be a positive multiple of 16", k);
+    DGB_REQUIRE(rows <= kMaxRows && k <= kMaxColumns, "rows (%d) or k (%d) too large", rows, k);
     DGB_REQUIRE(rows == 0 || (x != nullptr && q != nullptr && sf != nullptr), "null tensor pointer");
     DGB_REQUIRE(aligned_to(x, 16) && aligned_to(q, 16) && aligned_to(sf, 4) && x_row_stride % 8 == 0 && q_row_stride % 16 == 0,
                 "rows of x and q must be 16-byte aligned");
@@ -256,6 +260,7 @@ int check_plan(const int32_t* dest_row, const int32_t* expert_end, int tokens, i
     DGB_REQUIRE(tokens >= 0 && topk >= 1 && topk <= 32, "num_topk (%d) must be in [1, 32]", topk);
     DGB_REQUIRE(experts >= 1 && experts <= kMaxPlanExperts, "experts (%d) must be in [1, %d]", experts, kMaxPlanExperts);
     DGB_REQUIRE(alignment >= 1 && capacity >= 0, "alignment must be positive");
+    DGB_REQUIRE(alignment <= kMaxColumns, "alignment (%d) is too large", alignment);
     DGB_REQUIRE((dest_row != nullptr || tokens == 0) && expert_end != nullptr, "null tensor pointer");
     return 0;
 }
@@ -287,7 +292,7 @@ int run_unpermute(UnpermuteParams& p, bool backward, int is_fp32, cudaStream_t s
     if (const int rc = check_plan(p.dest_row, p.expert_end != nullptr || backward ? p.expert_end : p.dest_row, p.tokens, p.topk, p.experts, p.alignment,
                                   p.capacity))
         return rc;
-    DGB_REQUIRE(p.hidden >= 1, "hidden must be positive");
+    DGB_REQUIRE(p.hidden >= 1 && p.hidden <= kMaxColumns, "hidden (%d) must be in [1, %d]", p.hidden, kMaxColumns);
     const int es = is_fp32 ? 4 : 2;
     DGB_REQUIRE(p.out != nullptr || (backward ? p.capacity : p.tokens) == 0, "null output");
     DGB_REQUIRE(p.rows != nullptr || p.capacity == 0, "null tensor pointer");
@@ -315,6 +320,7 @@ int run_unpermute(UnpermuteParams& p, bool backward, int is_fp32, cudaStream_t s
 
 int check_swiglu(const SwigluParams& p, bool backward, int out_width, int out_es) {
     DGB_REQUIRE(p.rows >= 0 && p.inter >= 1, "rows must be >= 0 and inter positive");
+    DGB_REQUIRE(p.rows <= kMaxRows && p.inter <= kMaxColumns, "rows (%d) or inter (%d) too large", p.rows, p.inter);
     DGB_REQUIRE(p.rows == 0 || (p.x != nullptr && p.out != nullptr && (!backward || p.dy != nullptr)), "null tensor pointer");
     DGB_REQUIRE(p.layout == nullptr || (p.num_groups > 0 && p.alignment > 0), "a layout needs its groups and alignment");
     DGB_REQUIRE(p.x_stride >= 2ll * p.inter && p.out_stride >= out_width && (!backward || p.dy_stride >= p.inter), "row strides must cover the rows");
@@ -436,7 +442,7 @@ int dgb200_moe_dispatch_plan(const int64_t* topk_idx, int32_t num_tokens, int32_
     if (const int rc = check_plan(dest_row, expert_end, num_tokens, num_topk, num_experts, alignment, 0)) return rc;
     const long long entries = static_cast<long long>(num_tokens) * num_topk;
     DGB_REQUIRE((topk_idx != nullptr || entries == 0) && expert_start != nullptr, "null tensor pointer");
-    DGB_REQUIRE(entries + static_cast<long long>(num_experts) * (alignment - 1) < (1ll << 31), "too many rows");
+    DGB_REQUIRE(entries + static_cast<long long>(num_experts) * (alignment - 1) <= kMaxRows, "too many rows");
     const int chunk = sort_chunk_entries(entries);
     const int chunks = static_cast<int>((entries + chunk - 1) / chunk);
     DGB_REQUIRE(chunks <= 1 || (workspace != nullptr && aligned_to(workspace, 4)), "the plan needs its workspace");
@@ -524,7 +530,7 @@ int dgb200_moe_unpermute(const void* rows, int64_t rows_row_stride, const float*
     p.experts = 1;
     p.alignment = 1;
     p.capacity = capacity;
-    DGB_REQUIRE(num_tokens > 0 || num_tokens == 0, "num_tokens must be >= 0");
+    DGB_REQUIRE(num_tokens >= 0, "num_tokens must be >= 0");
     if (num_tokens == 0) return 0;
     return run_unpermute(p, false, is_fp32, static_cast<cudaStream_t>(stream));
 }

@@ -57,8 +57,10 @@ def _check_plan(plan: MoeDispatchPlan):
     experts = end.numel()
     if not 1 <= experts <= _MAX_EXPERTS or start.shape != end.shape:
         raise RuntimeError(f'the plan must hold 1 to {_MAX_EXPERTS} experts')
-    if alignment < 1:
+    if not 1 <= alignment < 2 ** 31:
         raise RuntimeError('the alignment must be positive')
+    if tokens >= 2 ** 31:
+        raise RuntimeError('the plan is too large')
     return tokens, topk, experts, _capacity(tokens * topk, experts, alignment)
 
 
@@ -72,6 +74,8 @@ def _check_rows(t: torch.Tensor, rows: Optional[int], width: Optional[int], dtyp
     if (rows is not None and height != rows) or (width is not None and columns != width) or columns == 0:
         raise RuntimeError(f'{name} has shape {(height, columns)}, expected ({rows if rows is not None else "any"}, '
                            f'{width if width is not None else "at least 1"})')
+    if height >= 2 ** 31 or columns >= 2 ** 31:
+        raise RuntimeError(f'{name} is too large')
     if height > 1 and row_stride < columns:
         raise RuntimeError(f'rows of {name} must not overlap')
 
@@ -98,11 +102,13 @@ def moe_dispatch_plan(topk_idx: torch.Tensor, num_experts: int, alignment: Optio
         raise RuntimeError('topk_idx must be a contiguous CUDA int64 [tokens, topk] tensor')
     alignment = get_mk_alignment_for_contiguous_layout() if alignment is None else int(alignment)
     tokens, topk = topk_idx.shape
+    if tokens >= 2 ** 31:
+        raise RuntimeError('topk_idx is too large')
     if not 1 <= topk <= _MAX_TOPK:
         raise RuntimeError(f'num_topk must be in [1, {_MAX_TOPK}]')
     if not 1 <= num_experts <= _MAX_EXPERTS:
         raise RuntimeError(f'num_experts must be in [1, {_MAX_EXPERTS}]')
-    if alignment < 1:
+    if not 1 <= alignment < 2 ** 31:
         raise RuntimeError('the alignment must be positive')
     lib = _lib.lib()
     workspace_bytes = lib.dgb200_moe_dispatch_plan_workspace_bytes(tokens, topk, num_experts)
@@ -124,7 +130,7 @@ def moe_permute(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], plan:
     tokens, topk, experts, capacity = _check_plan(plan)
     dest, end = plan.dest_row, plan.expert_end
     pair = isinstance(x, tuple)
-    if pair and (len(x) != 2 or (out is not None and (not isinstance(out, tuple) or len(out) != 2))):
+    if (pair and len(x) != 2) or (out is not None and (isinstance(out, tuple) != pair or (pair and len(out) != 2))):
         raise RuntimeError('x and out must both be pairs (rows, scales), or both tensors')
     q, sf = x if pair else (x, None)
     _check_rows(q, tokens, None, (torch.float8_e4m3fn,) if pair else (torch.bfloat16, torch.float32), 'x')

@@ -90,6 +90,8 @@ def _cast_f32_scales(x: torch.Tensor, gran_k: int) -> Tuple[torch.Tensor, torch.
     m, k = x.shape
     if k == 0 or k % 16 != 0 or gran_k not in (32, 128):
         raise RuntimeError(f'k ({k}) must be a positive multiple of 16 and gran_k ({gran_k}) 32 or 128')
+    if max(m, k) >= 2 ** 31:
+        raise RuntimeError('x is too large')
     if x.stride(1) != 1 or (m > 1 and (x.stride(0) < k or x.stride(0) % 8 != 0)) or x.data_ptr() % 16 != 0:
         x = x.clone(memory_format=torch.contiguous_format)
     with _lib.on_device(x.device):
@@ -111,6 +113,8 @@ def per_block_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128) -
     n, k = x.shape[-2:]
     if k == 0 or k % 16 != 0:
         raise RuntimeError(f'k ({k}) must be a positive multiple of 16')
+    if max(x.shape) >= 2 ** 31:
+        raise RuntimeError('x is too large')
     if x.stride(-1) != 1 or any(s % 8 != 0 or s < 0 for s in x.stride()[:-1]) or x.data_ptr() % 16 != 0 or (n > 1 and x.stride(-2) < k):
         x = x.clone(memory_format=torch.contiguous_format)
     groups = x.size(0) if x.dim() == 3 else 1

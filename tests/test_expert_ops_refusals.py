@@ -167,3 +167,51 @@ def test_python_refusals_on_the_gpu():
                         (lambda: dg.swiglu_per_token_cast_to_fp8(wide[:, :72]), 'multiple of 8'), (lambda: dg.swiglu(wide.t()), 'unit inner')):
         with pytest.raises(RuntimeError, match=match):
             call()
+
+
+LARGE = 2 ** 31 - 1  # counts of tiles, vectors and rows are 32-bit: sizes near their end are refused
+
+
+def test_sizes_near_the_end_of_32_bits(lib):
+    fields = dict(size=168, a=4096, sfa=4096, b=4096, sfb=4096, d=4096, c=0, layout=4096, sfa_group_stride=0, sfa_row_stride=1, sfa_k_stride=1,
+                  sfb_group_stride=0, sfb_n_stride=1, sfb_k_stride=1, d_row_stride=256, c_row_stride=256, m=64, n=256, k=256, num_groups=1,
+                  layout_kind=3, alignment=128, store_padding=0, expected_m=64, b_mn_major=0, d_is_fp32=0)
+    for change in (dict(m=LARGE), dict(n=2 ** 31 - 16, d_row_stride=2 ** 31), dict(k=2 ** 31 - 16)):
+        args = struct.pack('@N7P8q10i', *({**fields, **change}[f] for f in FIELDS))
+        refused(lib, lib.dgb200_fp8_block_scaled_gemm(args, NULL), 'too large')
+    refused(lib, lib.dgb200_per_token_cast_to_fp8_f32_scales(P, 16, LARGE, 16, 128, P, 16, P, 1, NULL), 'too large')
+    refused(lib, lib.dgb200_moe_dispatch_plan(P, LARGE, 1, 1, 1, P, P, P, P, NULL), 'too many')
+    refused(lib, lib.dgb200_moe_dispatch_plan(P, 1, 1, 1, LARGE, P, P, P, NULL, NULL), 'alignment')
+    refused(lib, lib.dgb200_moe_permute(P, 128, 128, P, 128, NULL, 0, 0, NULL, 0, P, P, 0, 1, 1, LARGE, 4, 1, NULL), 'alignment')
+    refused(lib, lib.dgb200_moe_unpermute(P, 2 ** 31, P, P, P, 2 ** 31, 4, 2, LARGE, 100, 0, NULL), 'hidden')
+    refused(lib, lib.dgb200_swiglu(P, 2 ** 32, P, 2 ** 31, 4, LARGE, NULL, 0, 0, 0.0, NULL), 'too large')
+    refused(lib, lib.dgb200_swiglu_backward(P, 64, P, 128, P, 128, LARGE, 64, NULL, 0, 0, 0.0, NULL), 'too large')
+
+
+def test_python_refuses_sizes_beyond_32_bits(monkeypatch):
+    # a row that repeats stands for a buffer of that many rows
+    for t in (torch.zeros(1, 1).expand(2 ** 31, 1), torch.zeros(1, 1).expand(1, 2 ** 31)):
+        monkeypatch.setattr(torch.Tensor, 'is_cuda', True)
+        from deepgemm_b200.permute import _check_rows
+        with pytest.raises(RuntimeError, match='too large|inner stride'):
+            _check_rows(t, None, None, (torch.float32,), 'out')
+    with pytest.raises(RuntimeError, match='too large'):
+        dg.utils.per_token_cast_to_fp8(torch.zeros(1, 16, dtype=torch.bfloat16).expand(2 ** 31, 16), use_ue8m0=False)
+    with pytest.raises(RuntimeError, match='too large'):
+        dg.utils.per_block_cast_to_fp8(torch.zeros(1, 16, dtype=torch.bfloat16).expand(2 ** 31, 16), use_ue8m0=False)
+    with pytest.raises(RuntimeError, match='too large'):
+        dg.moe_dispatch_plan(torch.zeros(2 ** 31, 0, dtype=torch.int64), 8)
+
+
+@pytest.mark.gpu
+def test_more_python_refusals_on_the_gpu():
+    plan = dg.moe_dispatch_plan(torch.zeros(5, 2, dtype=torch.int64, device='cuda'), 4, alignment=8)
+    x = torch.zeros(5, 64, dtype=torch.bfloat16, device='cuda')
+    rows = torch.zeros(plan.capacity, 64, dtype=torch.bfloat16, device='cuda')
+    with pytest.raises(RuntimeError, match='pairs'):
+        dg.moe_permute(x, plan, out=(rows, rows))
+    store = torch.zeros(128 * 128 * 2 + 16, dtype=torch.uint8, device='cuda')
+    d, layout = store[:128 * 128 * 2].view(torch.bfloat16).view(128, 128), store[256:260].view(torch.int32)
+    a, sfa = torch.zeros(128, 128, device='cuda').to(torch.float8_e4m3fn), torch.ones(128, 1, device='cuda')
+    with pytest.raises(RuntimeError, match='overlap'):
+        dg.m_grouped_fp8_gemm_nt_contiguous((a, sfa), (a[None], sfa[None, :1]), d, layout, disable_ue8m0_cast=True, use_psum_layout=True)
