@@ -35,7 +35,7 @@ __device__ __forceinline__ int swiglu_rows(const SwigluParams& p) {
 __device__ __forceinline__ float clamp_above(float v, float c) { return v > c ? c : v; }
 __device__ __forceinline__ float clamp_both(float v, float c) { return v > c ? c : (v < -c ? -c : v); }
 
-// 1 / (1 + e^-x) from the hardware's exponential and reciprocal: about 2^-22 off, far below the BF16 or E4M3 rounding that follows.
+// 1 / (1 + e^-x) from the hardware's exponential and reciprocal: about 2^-22 off, far below the BF16 rounding that follows.
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_approx(1.0f + __expf(-x)); }
 
 // One thread: kVec columns of kRows consecutive rows, so that 2 kRows loads (3 kRows backward) are in flight.
