@@ -445,6 +445,8 @@ int dgb200_moe_dispatch_plan(const int64_t* topk_idx, int32_t num_tokens, int32_
     DGB_REQUIRE(entries + static_cast<long long>(num_experts) * (alignment - 1) <= kMaxRows, "too many rows");
     const int chunk = sort_chunk_entries(entries);
     const int chunks = static_cast<int>((entries + chunk - 1) / chunk);
+    // the kernels form the end of a chunk in 32 bits: above 0x7ffe0000 entries the last one's would be 2^31
+    DGB_REQUIRE(static_cast<long long>(chunks) * chunk < (1ll << 31), "too many entries");
     DGB_REQUIRE(chunks <= 1 || (workspace != nullptr && aligned_to(workspace, 4)), "the plan needs its workspace");
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     if (entries <= kPlanThreads) {

@@ -519,7 +519,8 @@ int dgb200_per_block_cast_to_fp8(const void* x, int64_t x_group_stride, int64_t 
  *   expert_start, expert_end  int32 [num_experts]: the segments; each starts at a multiple of `alignment`. expert_end is the psum
  *             layout of the grouped GEMMs (of the same alignment).
  *   workspace dgb200_moe_dispatch_plan_workspace_bytes(...) bytes of device memory (0: may be NULL); calls that may overlap need one each.
- * num_topk <= 32, num_experts <= 1024. */
+ * num_topk <= 32, num_experts <= 1024, num_tokens * num_topk <= 0x7ffe0000, and the rows with their padding (num_tokens * num_topk +
+ * num_experts * (alignment - 1)) <= 0x7ffff000. */
 int64_t dgb200_moe_dispatch_plan_workspace_bytes(int32_t num_tokens, int32_t num_topk, int32_t num_experts);
 int dgb200_moe_dispatch_plan(const int64_t* topk_idx, int32_t num_tokens, int32_t num_topk, int32_t num_experts, int32_t alignment,
                              int32_t* dest_row, int32_t* expert_start, int32_t* expert_end, void* workspace, void* stream);
