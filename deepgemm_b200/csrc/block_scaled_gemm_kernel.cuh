@@ -429,6 +429,8 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
             while (ok && sched.next(t)) {
                 if (t.group < 0) continue;
                 const long long group = t.group;
+                // rows with scales: padding rows that are stored have none (a zero there keeps what their words hold out of d)
+                const int scaled_rows = p.store_padding ? min(t.rows, __ldg(p.layout + t.group) - t.row0) : t.rows;
                 const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + static_cast<long long>(t.row0 + static_cast<int>(lane)) * p.sfa_row_stride;
                 // B's scales are the same for all rows: lane 4 h + i loads the one of half h and K block i of the four
                 const float* sfb = p.sfb + group * p.sfb_group_stride +
@@ -440,7 +442,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
 #pragma unroll
                     for (int j = 0; j < 4; ++j)  // rows that are not stored need no scale: none is read for them
                         load_scales(sfa + 32 * j * p.sfa_row_stride + kb * p.sfa_k_stride, p.sfa_k_stride,
-                                    static_cast<int>(lane) + 32 * j < t.rows ? num_kb - kb : 0, whole, a[j]);
+                                    static_cast<int>(lane) + 32 * j < scaled_rows ? num_kb - kb : 0, whole, a[j]);
                     const float b = static_cast<int>(lane % kScaleKb) < num_kb - kb ? __ldg(sfb + kb * p.sfb_k_stride) : 0.0f;
 #pragma unroll
                     for (int i = 0; i < kScaleKb; ++i) {

@@ -152,7 +152,7 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     p.k = a.k;
     p.num_groups = a.num_groups;
     p.alignment = dense || masked ? 128 : a.alignment;
-    p.store_padding = a.store_padding;
+    p.store_padding = psum && a.store_padding;
     p.b_mn_major = a.b_mn_major ? 1 : 0;
     p.sf_vec = a.sfa_k_stride == 1 && aligned_to(a.sfa, 16) && a.sfa_row_stride % 4 == 0 && a.sfa_group_stride % 4 == 0;
     int sms = 0;

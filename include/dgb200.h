@@ -478,8 +478,8 @@ int dgb200_moe_dispatch_plan_noalloc(const int64_t* topk_idx, int32_t num_tokens
  *   d    bf16, or float with d_is_fp32, row stride d_row_stride elements; rows 16-byte aligned.
  *   c    optional (dense form, float d): float [m, n], may be d itself with the same stride, must not overlap it otherwise.
  *   layout, layout_kind, alignment, store_padding, expected_m (masked: steers tiling only): as in the GEMMs above. Rows outside
- *        the groups are not written, save for padding rows with store_padding (psum) and the rest of a started 128-row tile (row
- *        ids). Layout words that name rows past m, or groups that do not exist, are cut off there (row ids: reported in the status block).
+ *        the groups are not written, save for padding rows with store_padding (psum; the scales of padding rows count as zero and are
+ *        not read, so those rows of d are zero unless a holds NaN there) and the rest of a started 128-row tile (row ids). Layout words that name rows past m, or groups that do not exist, are cut off there (row ids: reported in the status block).
  * n % 8 == 0, k % 16 == 0 (last blocks may be short), at most 512 groups in the psum and masked layouts; a and b 16-byte aligned. */
 typedef struct dgb200_fp8_block_scaled_gemm_args {
     size_t struct_size; /* sizeof(dgb200_fp8_block_scaled_gemm_args) */
