@@ -143,7 +143,7 @@ struct BlockScaledSmem {
     static constexpr int kNumBars = 2 * kStages + kAccums;
     static constexpr int kOffMisc = kOffBar + (kNumBars * 8 + 15) / 16 * 16;
     static constexpr int kOffGroups = kOffMisc + 16;
-    static constexpr int kTotal = kOffGroups + 3 * kMaxCachedGroups * 4;
+    static constexpr int kTotal = kOffGroups + 4 * kMaxCachedGroups * 4;
     static constexpr int kDynamicBytes = kTotal + 1024;  // slack to align the base to 1024 B
 };
 
@@ -155,7 +155,7 @@ struct BlockScaledTile {
 };
 
 // Walks the output tiles. Groups come from the table that the prologue puts into shared memory: start row, rows to
-// compute and running tile count of each.
+// compute, running tile count and end of the rows with scales of each.
 // `ctas`: CTAs that share a tile (a pair, or a cluster that splits the tile's K).
 template <int BLOCK_N, bool kPair>
 struct BlockScaledScheduler {
@@ -181,10 +181,11 @@ struct BlockScaledScheduler {
     }
 
     // Rows of a group from the layout words; whatever they hold, no row at or past p.m is named.
-    __device__ __forceinline__ static void group_extent(const BlockScaledParams& p, int group, int& first, int& count) {
+    // `scaled`: end of the rows that have scales, in front of the padding rows among the `count`.
+    __device__ __forceinline__ static void group_extent(const BlockScaledParams& p, int group, int& first, int& count, int& scaled) {
         if (p.mode == kModeMasked) {
             first = 0;
-            count = min(max(__ldg(p.layout + group), 0), p.m);
+            count = scaled = min(max(__ldg(p.layout + group), 0), p.m);
             return;
         }
         const int prev_end = group == 0 ? 0 : min(max(__ldg(p.layout + group - 1), 0), p.m);
@@ -193,6 +194,7 @@ struct BlockScaledScheduler {
         first = static_cast<int>(min((prev_end + al - 1) / al * al, static_cast<long long>(p.m)));
         const int last = p.store_padding ? static_cast<int>(min((end + al - 1) / al * al, static_cast<long long>(p.m))) : end;
         count = end > first ? last - first : 0;
+        scaled = end;
     }
 
     __device__ bool next(BlockScaledTile& t) {
@@ -278,10 +280,11 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
     if (p.mode == kModePsum || p.mode == kModeMasked) {
         int* tiles_end = table + 2 * kMaxCachedGroups;
         for (int i = threadIdx.x; i < p.num_groups; i += kThreads) {
-            int first, count;
-            Sched::group_extent(p, i, first, count);
+            int first, count, scaled;
+            Sched::group_extent(p, i, first, count, scaled);
             table[i] = first;
             table[kMaxCachedGroups + i] = count;
+            table[3 * kMaxCachedGroups + i] = scaled;
             tiles_end[i] = (count + Sched::kTileM - 1) / Sched::kTileM * ((p.n + BLOCK_N - 1) / BLOCK_N);
         }
         __syncthreads();
@@ -430,7 +433,7 @@ dgb200_block_scaled_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const 
                 if (t.group < 0) continue;
                 const long long group = t.group;
                 // rows with scales: padding rows that are stored have none (a zero there keeps what their words hold out of d)
-                const int scaled_rows = p.store_padding ? min(t.rows, __ldg(p.layout + t.group) - t.row0) : t.rows;
+                const int scaled_rows = p.store_padding ? min(t.rows, table[3 * kMaxCachedGroups + t.group] - t.row0) : t.rows;
                 const float* sfa = p.sfa + (p.mode == kModeMasked ? group * p.sfa_group_stride : 0) + static_cast<long long>(t.row0 + static_cast<int>(lane)) * p.sfa_row_stride;
                 // B's scales are the same for all rows: lane 4 h + i loads the one of half h and K block i of the four
                 const float* sfb = p.sfb + group * p.sfb_group_stride +
