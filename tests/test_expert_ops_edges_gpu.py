@@ -44,3 +44,62 @@ def test_padding_rows_are_zero_whatever_their_scales_hold(dg, form, nn):
         for knob, value in (('block_n', 0), ('pair', -1)):
             _lib.check(_lib.lib().dgb200_set_tuning(knob.encode(), value))
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ------------------------------------------------------------------------------------------------------- gates far below zero
+# The sigmoid's relative error there is the exponential's: 2 + 1.16 |g| half steps (2^-24 each, the documented bound of the fast one is in whole
+# ones) and a few roundings: (1.16 |g| + 12) * 2^-23 of the value, or of the terms of the gate's gradient. One rounding to BF16.
+
+def far_case(inter, seed):
+    """Gates from 0 to -170 in every step of BF16 that lies there, with values of `up` that keep the product among ordinary numbers."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    gate = torch.cat([torch.arange(-170.0, -60.0, 0.5), torch.arange(-60.0, 0.0, 0.25)])
+    gate = gate.bfloat16().unique().cuda()
+    gate = gate[torch.randint(0, gate.numel(), (64, inter), generator=g, device='cuda')]
+    size = torch.exp2((-gate.float() * 1.4427).clamp(max=118.0) + torch.rand(64, inter, generator=g, device='cuda') * 6 - 3)
+    up = (size * torch.where(torch.rand(64, inter, generator=g, device='cuda') < 0.5, -1.0, 1.0)).bfloat16()
+    dy = torch.randn(64, inter, generator=g, device='cuda').bfloat16()
+    return torch.cat([gate, up], dim=1), dy
+
+
+def far_reference(x, dy):
+    inter = x.shape[1] // 2
+    g, u, dy = x[:, :inter].double(), x[:, inter:].double(), dy.double()
+    s = torch.exp(g) / (1 + torch.exp(g))
+    return g * s * u, dy * u * s * (1 + g * (1 - s)), dy * g * s, dy.abs() * u.abs() * s * (1 + g.abs())
+
+
+@pytest.mark.parametrize('inter', [7, 264])
+@pytest.mark.parametrize('clamp', [None, 3e38])
+def test_gates_far_below_zero(dg, inter, clamp):
+    x, dy = far_case(inter, seed=3)
+    y, d_gate, d_up, terms = far_reference(x, dy)
+    error = (1.16 * x[:, :inter].double().abs() + 12) * 2.0 ** -23
+    smallest = 2.0 ** -134  # half a step of BF16's subnormal numbers
+    got = dg.swiglu(x, activation_clamp=clamp).double()
+    assert ((got - y).abs() <= y.abs() * (2.0 ** -8 + error) + smallest).all()
+    got = dg.swiglu_backward(dy, x, activation_clamp=clamp).double()
+    assert ((got[:, :inter] - d_gate).abs() <= d_gate.abs() * 2.0 ** -8 + terms * error * 1.01 + smallest).all()
+    assert ((got[:, inter:] - d_up).abs() <= d_up.abs() * (2.0 ** -8 + error) + smallest).all()
+    if inter % 8 == 0:
+        q, sf = dg.swiglu_per_token_cast_to_fp8(x, activation_clamp=clamp)
+        blocks = -(-inter // 128)
+        amax = torch.nn.functional.pad(y, (0, blocks * 128 - inter)).view(64, blocks, 128).abs().amax(dim=-1)
+        scale = amax.clamp(min=1e-4) / 448
+        assert ((sf.double() - scale).abs() <= scale * 2.0 ** -19).all()
+        wide = sf.double().repeat_interleave(128, dim=1)[:, :inter]
+        step = torch.maximum(y.abs() * 2.0 ** -4, wide * 2.0 ** -10)
+        assert ((q.double() * wide - y).abs() <= step * 1.001 + y.abs() * 2.0 ** -18).all()
+
+
+def test_a_gate_at_the_end_of_the_exponential(dg):
+    """-87.5 and 1e36: the denominator of the sigmoid is finite, its reciprocal no normal number; the product is about -0.87."""
+    for g in (-87.0, -87.5, -88.0, -88.5, -89.0, -104.0):
+        x = torch.tensor([[g] * 8 + [1e36] * 8], dtype=torch.float64)
+        want = g * torch.exp(torch.tensor(g, dtype=torch.float64)) * float(x.bfloat16()[0, 8])
+        x = x.bfloat16().cuda()
+        assert abs(float(dg.swiglu(x)[0, 0]) - float(want)) <= abs(float(want)) * 2.0 ** -7
+        q, sf = dg.swiglu_per_token_cast_to_fp8(x)
+        assert abs(float(q.float()[0, 0] * sf[0, 0]) - float(want)) <= max(abs(float(want)) * 2.0 ** -4, 1e-4 / 448 * 2.0 ** -10) * 1.01
+    x = torch.tensor([[-float('inf')] * 8 + [2.0] * 8], device='cuda').bfloat16()
+    assert torch.isnan(dg.swiglu(x)).all() and torch.isnan(dg.swiglu_per_token_cast_to_fp8(x)[0].float()).all()  # infinity times zero
