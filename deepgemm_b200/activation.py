@@ -1,5 +1,6 @@
 """SwiGLU of the experts' rows as operators of their own, forward (to BF16, or straight to FP8 with FP32 scales) and backward, for callers
 that run the grouped GEMMs themselves; the Mega-MoE layers fuse the forward form into their gate/up GEMM."""
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -18,7 +19,7 @@ def _check_call(gate_up, grouped_layout, activation_clamp):
     if grouped_layout is not None and not (grouped_layout.is_cuda and grouped_layout.dtype == torch.int32 and grouped_layout.dim() == 1 and
                                            grouped_layout.is_contiguous() and grouped_layout.numel() > 0):
         raise RuntimeError('grouped_layout must be a contiguous CUDA int32 tensor, one end row per group')
-    if activation_clamp is not None and not activation_clamp > 0:
+    if activation_clamp is not None and not ctypes.c_float(activation_clamp).value > 0:  # in FP32, where zero stands for no clamp
         raise RuntimeError('activation_clamp must be positive (None: no clamp)')
     layout = (grouped_layout.data_ptr(), grouped_layout.numel(), get_mk_alignment_for_contiguous_layout()) if grouped_layout is not None else (None, 0, 0)
     return gate_up.size(0), gate_up.size(1) // 2, layout + (float(activation_clamp) if activation_clamp is not None else 0.0,)

@@ -103,3 +103,14 @@ def test_a_gate_at_the_end_of_the_exponential(dg):
         assert abs(float(q.float()[0, 0] * sf[0, 0]) - float(want)) <= max(abs(float(want)) * 2.0 ** -4, 1e-4 / 448 * 2.0 ** -10) * 1.01
     x = torch.tensor([[-float('inf')] * 8 + [2.0] * 8], device='cuda').bfloat16()
     assert torch.isnan(dg.swiglu(x)).all() and torch.isnan(dg.swiglu_per_token_cast_to_fp8(x)[0].float()).all()  # infinity times zero
+
+
+def test_a_clamp_that_fp32_rounds_to_zero_is_refused(dg):
+    x = torch.ones(2, 32, dtype=torch.bfloat16, device='cuda')
+    for call in (lambda c: dg.swiglu(x, activation_clamp=c), lambda c: dg.swiglu_backward(x[:, :16], x, activation_clamp=c),
+                 lambda c: dg.swiglu_per_token_cast_to_fp8(x, activation_clamp=c)):
+        for c in (1e-46, 1e-300):
+            with pytest.raises(RuntimeError, match='positive'):
+                call(c)
+    assert (dg.swiglu(x, activation_clamp=1e-44).float() == 0).all()  # the smallest clamps still hold
+    assert torch.equal(dg.swiglu(x, activation_clamp=1e300), dg.swiglu(x))
