@@ -115,6 +115,6 @@ def run(a, b, d, c, layout, layout_kind, recipe, recipe_a, recipe_b, alignment=1
         layout.data_ptr() if layout is not None else 0, a_sf.stride(0) if masked else 0, a_sf.stride(-2), a_sf.stride(-1),
         0 if dense else b_sf.stride(0), b_sf.stride(-2), b_sf.stride(-1), row_stride,
         (c.stride(-2) if m > 1 else n) if c is not None else 0, m, n, k, groups, layout_kind, alignment,
-        int(bool(store_padding)), int(expected_m), int(b_mn_major), int(d.dtype == torch.float32))
+        int(bool(store_padding)), min(int(expected_m), m), int(b_mn_major), int(d.dtype == torch.float32))
     with _lib.on_device(d.device):
         _lib.check(_lib.lib().dgb200_fp8_block_scaled_gemm(args, _lib.current_stream_ptr()))

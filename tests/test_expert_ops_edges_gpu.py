@@ -114,3 +114,17 @@ def test_a_clamp_that_fp32_rounds_to_zero_is_refused(dg):
                 call(c)
     assert (dg.swiglu(x, activation_clamp=1e-44).float() == 0).all()  # the smallest clamps still hold
     assert torch.equal(dg.swiglu(x, activation_clamp=1e300), dg.swiglu(x))
+
+
+def test_expected_rows_beyond_32_bits_only_steer(dg):
+    g = torch.Generator(device='cuda').manual_seed(5)
+    a = torch.randint(0, 0x70, (3, 40, 256), generator=g, device='cuda', dtype=torch.uint8).view(torch.float8_e4m3fn)
+    b = torch.randint(0, 0x70, (3, 128, 256), generator=g, device='cuda', dtype=torch.uint8).view(torch.float8_e4m3fn)
+    sfa, sfb = torch.rand(3, 40, 2, generator=g, device='cuda'), torch.rand(3, 1, 2, generator=g, device='cuda')
+    counts = torch.tensor([40, 0, 7], dtype=torch.int32, device='cuda')
+    outs = []
+    for expected in (40, 2 ** 31, 2 ** 40):
+        d = torch.zeros(3, 40, 128, dtype=torch.bfloat16, device='cuda')
+        dg.m_grouped_fp8_gemm_nt_masked((a, sfa), (b, sfb), d, counts, expected, disable_ue8m0_cast=True)
+        outs.append(d)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and (outs[0][0] != 0).any()
