@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(256) dgb200_cast_rows_nvfp4_kernel(const CastN
 // rounds it. The quotient comes from the correctly rounded reciprocal y by one residual step (Markstein, as in
 // e2m1_codes_of_quotients): |sf| lies in [2^-23, 2^120], so that neither the reciprocal nor a quotient that E4M3 can hold leaves the normal range.
 // NaN stays NaN and is passed over by the maximum; a block that holds an infinity has the scale infinity, its infinities become
-// NaN and the rest zero, as the division gives.
+// NaN and the rest zero, as the division gives. With a power of two as the scale it is 2^127, the largest there is, for such a block, and
+// its infinities take the largest code (as in dgb200_cast_rows_kernel), whose product with the scale is infinite again.
 // ------------------------------------------------------------------------------------------------------------------
 // The quotients are formed with the sign turned, two at a time, and turned back in the codes: with y' = -1/sf the steps are q' = v y',
 // r = v + q' sf, q' + r y', and a zero comes out with v's sign (the other way round a residual of +0 would make +0 of -0).

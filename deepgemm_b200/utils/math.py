@@ -104,7 +104,8 @@ def _cast_f32_scales(x: torch.Tensor, gran_k: int) -> Tuple[torch.Tensor, torch.
 
 def per_block_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool, gran_k: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
     """x bfloat16 [N, K], or [G, N, K] for the weights of G experts -> (e4m3 of that shape, fp32 [.., ceil(N / 128), ceil(K / 128)]), one scale
-    per 128 x 128 block: max(amax, 1e-4) / 448, or the smallest power of two not below it. K must be a multiple of 16.
+    per 128 x 128 block: max(amax, 1e-4) / 448, or the smallest power of two not below it (at most 2^127, which a block with an infinity
+    has). K must be a multiple of 16.
     Reference: per_block_cast_to_fp8, deep_gemm/utils/math.py:62-73."""
     if gran_k != 128:
         raise RuntimeError('blocks are 128 x 128: gran_k must be 128')

@@ -506,7 +506,8 @@ int dgb200_per_token_cast_to_fp8_f32_scales(const void* x, int64_t x_row_stride,
                                             int64_t q_row_stride, float* sf, int64_t sf_row_stride, void* stream);
 
 /* BF16 [num_groups, rows, k] -> E4M3 + one FP32 scale per 128 x 128 block (edge blocks may be short), rounded as above; use_ue8m0 != 0: the
- * scale is the smallest power of two not below it. Reference: per_block_cast_to_fp8, deep_gemm/utils/math.py:62-73. */
+ * scale is the smallest power of two not below it, at most 2^127 (a block that holds an infinity: its infinities become +-448, the rest 0).
+ * Reference: per_block_cast_to_fp8, deep_gemm/utils/math.py:62-73. */
 int dgb200_per_block_cast_to_fp8(const void* x, int64_t x_group_stride, int64_t x_row_stride, int32_t num_groups, int32_t rows, int32_t k,
                                  int32_t use_ue8m0, void* q, int64_t q_group_stride, int64_t q_row_stride, float* sf, int64_t sf_group_stride,
                                  int64_t sf_row_stride, void* stream);

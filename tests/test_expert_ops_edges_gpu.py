@@ -128,3 +128,26 @@ def test_expected_rows_beyond_32_bits_only_steer(dg):
         dg.m_grouped_fp8_gemm_nt_masked((a, sfa), (b, sfb), d, counts, expected, disable_ue8m0_cast=True)
         outs.append(d)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and (outs[0][0] != 0).any()
+
+
+@pytest.mark.parametrize('special', ['inf', '-inf', 'nan'])
+def test_special_values_in_blocks_with_a_power_of_two_scale(dg, special):
+    """As the per-token quantiser with power-of-two scales: a block with an infinity has the largest scale, 2^127, and its infinities the largest
+    code, whose product with the scale is infinite; NaN stays NaN and is passed over by the maximum."""
+    x = torch.ones(130, 272, dtype=torch.bfloat16, device='cuda')
+    x[5, 130] = float(special)
+    q, sf = dg.utils.per_block_cast_to_fp8(x, use_ue8m0=True)
+    if special == 'nan':
+        assert torch.isnan(q[5, 130].float()) and (sf == 2.0 ** -8).all()
+        q.view(torch.uint8)[5, 130] = q.view(torch.uint8)[5, 131]
+        assert (q.float() == 256).all()
+        return
+    assert float(sf[0, 1]) == 2.0 ** 127 and float(q[5, 130].float()) == (448 if special == 'inf' else -448)
+    assert torch.isinf(q[5, 130].float() * sf[0, 1])
+    block = q[:128, 128:256].float().clone()
+    block[5, 2] = 0
+    assert (block == 0).all()
+    sf[0, 1] = 2.0 ** -8
+    assert (sf == 2.0 ** -8).all() and (q[:, :128].float() == 256).all() and (q[128:].float() == 256).all() and (q[:, 256:].float() == 256).all()
+    t, t_sf = dg.utils.per_token_cast_to_fp8(x[5:6, 128:256], use_ue8m0=True)
+    assert float(t_sf[0, 0]) == 2.0 ** 127 and torch.equal(t.view(torch.uint8)[0], q.view(torch.uint8)[5, 128:256])
