@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
 
 from deepgemm_b200 import _lib, build
+from deepgemm_b200.permute import _check_rows
 
 P, NULL = ctypes.c_void_p(4096), None
 
@@ -36,3 +38,13 @@ def test_no_chunk_of_the_sort_ends_past_32_bits(lib):
         assert chunks * entries_of == 2 ** 31
         refused(lib, lib.dgb200_moe_dispatch_plan(P, entries, 1, 1, 1, P, P, P, P, NULL), 'too many entries')
     refused(lib, lib.dgb200_moe_dispatch_plan(P, 0x7ffe0000 // 8 + 1, 8, 256, 1, P, P, P, P, NULL), 'too many entries')
+
+
+@pytest.mark.parametrize('shape', [(2 ** 31, 1), (1, 2 ** 31), (1, 2 ** 31 + 5)])
+def test_rows_and_columns_beyond_32_bits(monkeypatch, shape):
+    """Tensors of unit inner stride, so that nothing but their size can be refused."""
+    large, largest = torch.empty(shape, device='meta'), torch.empty(tuple(min(n, 2 ** 31 - 1) for n in shape), device='meta')
+    monkeypatch.setattr(torch.Tensor, 'is_cuda', True)
+    with pytest.raises(RuntimeError, match='x is too large'):
+        _check_rows(large, None, None, (torch.float32,), 'x')
+    _check_rows(largest, None, None, (torch.float32,), 'x')

@@ -151,3 +151,23 @@ def test_special_values_in_blocks_with_a_power_of_two_scale(dg, special):
     assert (sf == 2.0 ** -8).all() and (q[:, :128].float() == 256).all() and (q[128:].float() == 256).all() and (q[:, 256:].float() == 256).all()
     t, t_sf = dg.utils.per_token_cast_to_fp8(x[5:6, 128:256], use_ue8m0=True)
     assert float(t_sf[0, 0]) == 2.0 ** 127 and torch.equal(t.view(torch.uint8)[0], q.view(torch.uint8)[5, 128:256])
+
+
+def test_the_plan_with_the_most_chunks(dg):
+    """128 chunks, the last one full, short by one entry and of one entry."""
+    from deepgemm_b200 import _lib
+    experts, alignment = 300, 16
+    for entries in (6 * 131072, 6 * 131072 - 1, 127 * 6144 + 1):
+        assert _lib.lib().dgb200_moe_dispatch_plan_workspace_bytes(entries, 1, experts) == 128 * experts * 4
+        g = torch.Generator(device='cuda').manual_seed(entries)
+        flat = torch.randint(-1, experts, (entries,), generator=g, device='cuda')
+        plan = dg.moe_dispatch_plan(flat[:, None], experts, alignment=alignment)
+        order = torch.argsort(torch.where(flat < 0, experts, flat), stable=True)
+        counts = torch.bincount(flat[flat >= 0], minlength=experts)
+        padded = (counts + alignment - 1) // alignment * alignment
+        start, first = padded.cumsum(0) - padded, counts.cumsum(0) - counts
+        want = torch.full((entries,), -1, dtype=torch.int64, device='cuda')
+        kept = order[:int(counts.sum())]
+        want[kept] = start[flat[kept]] + torch.arange(kept.numel(), device='cuda') - first[flat[kept]]
+        assert torch.equal(plan.dest_row.flatten().long(), want)
+        assert torch.equal(plan.expert_start.long(), start) and torch.equal(plan.expert_end.long(), start + counts)
