@@ -1,8 +1,8 @@
 // SwiGLU of the experts' rows, forward and backward, as operators of their own (the layers fuse the forward form into their
 // gate/up GEMM). Rows are [gate | up]; with a clamp c the gate is min(gate, c) and up is clamped to [-c, c], and the
 // gradient is zero where a clamp holds. Bound by HBM: every value is read and written once in 16-byte vectors, four rows a thread where
-// there are many (32768 x 2 x 2048: forward 60.5 us, 6.65 TB/s; forward and backward over 64 segments 179 us, 36864 rows at most; to FP8 64.5 us,
-// 5.2 TB/s, where the issue slots are taken).
+// there are many (32768 x 2 x 2048, call after call: forward 61.5 us, 6.5 TB/s, backward 100.5, 6.7; to FP8 71 us, with a clamp 81, where the issue
+// slots are taken).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -42,8 +42,9 @@ __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_approx(1.0f 
 
 // Gates below kFarGate (e^87 lies under 2^126): 1 + e^g is one in FP32 and s = e^g = t^2 with t = e^(g / 2), a factor for each of the two
 // others, so that nothing leaves the normal range that the product does not. They are rare, so the BF16 kernels look for them with a minimum over all of
-// a thread's gates and mend what they gave behind the stores, in a function of its own. 32768 x 2 x 2048, forward and backward without any of it
-// 62.7 and 102.7 us; as it is 63.6 and 104.7; with the function inlined 65 and 108.5; with every gate's root selected in line 71 and 119.
+// a thread's gates and mend what they gave behind the stores, in a function of its own. 32768 x 2 x 2048 at a low clock, forward and backward
+// without any of it 62.7 and 102.7 us; as it is 63.6 and 104.7; with the function inlined 65 and 108.5; with every gate's root selected in line
+// 71 and 119 (at a high clock as it is and without: 61.5 and 100.5 both).
 constexpr float kFarGate = -87.0f;
 __device__ __forceinline__ float far_product(float a, float b, float t) { return (a * t) * (b * t); }
 
@@ -237,7 +238,7 @@ __device__ __forceinline__ void swiglu_cast_special_row(const SwigluParams& p, i
 // million was another). A lane owns 8 columns, 16 lanes a scale block; inter is a multiple of 8, a last block may be short. The issue slots
 // bound it: 32768 x 2 x 2048 59.4 us with the approximate operations, 69.0 with these, 64.5 with the divisions shared out among a block's lanes.
 // Where the maximum of a block is no finite number, the warp's rows are done one by one instead: far gates and NaN pass through the maxima, an
-// infinity may be the factor's. That costs 1 % where it is never taken (with a clamp, cold caches: 81.0 -> 82.0 us); finding far gates by a minimum, 5 %.
+// infinity may be the factor's. That costs 1 % where it is never taken (69.8 -> 71 us, with a clamp 80.0 -> 80.9); finding far gates by a minimum, 5 %.
 template <int kRows>
 __global__ void __launch_bounds__(256) dgb200_swiglu_cast_kernel(const SwigluParams p) {
     static_assert(kRows == 1 || kRows == 4, "lane l of a block divides for row l % kRows");

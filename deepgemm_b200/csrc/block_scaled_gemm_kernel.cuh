@@ -226,7 +226,8 @@ struct BlockScaledScheduler {
     }
 };
 
-constexpr int kRegsBsControl = 72, kRegsBsSum = 216;  // 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with
+// 128 x 72 + 256 x 216 = 384 x 168, what the block is launched with (the 256-wide forms spill one word)
+constexpr int kRegsBsControl = 72, kRegsBsSum = 216;
 
 // kSplitK (dense form): the CTAs of a cluster (2, 4 or 8) share one tile and take a part of its K blocks each; every CTA leaves its sums in its
 // own shared memory (the operand ring is done with), then the cluster adds them up, rank by rank in a fixed order. For problems

@@ -85,8 +85,8 @@ int launch_block_scaled_split(const CUtensorMap& tm_a, const CUtensorMap& tm_b, 
     return 0;
 }
 
-// CTAs per tile of a dense GEMM (1: no split): the largest of 8, 4 and 2 for which all clusters run at once and every part keeps at least 12
-// K blocks. Device time of calls back to back, no split -> split (us): 7 x 4096 x 7168 15.7 -> 11.0 (4), 33 x 1536 x 7168 15.1 -> 10.5
+// CTAs per tile of a dense GEMM (1: no split): the largest of 8, 4 and 2 for which all clusters run at once and every part gets at least three
+// groups of kScaleKb K blocks, 12 or, where the last group is short, 9. Device time of calls back to back, no split -> split (us): 7 x 4096 x 7168 15.7 -> 11.0 (4), 33 x 1536 x 7168 15.1 -> 10.5
 // (4; 8: 11.1), 512 x 2112 x 7168 16.3 -> 15.4 (2), 128 x 7168 x 16384 35.1 -> 29.4 (2). With less K it does not pay: 1 x 7168 x 2048 7.2 -> 7.8
 // (2), 64 x 7168 x 2048 7.5 -> 9.3 (2), 128 x 4096 x 2048 7.0 -> 9.6 (2).
 int block_scaled_split(long long tiles, int num_kb, bool f32, int sms, int* split) {
@@ -166,7 +166,11 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     // The tile width whose waves take the least time: a K block of a 256-, 128-, 64- or 32-wide tile takes about 540, 310, 260 or 240 ns, the
     // narrow ones because a K block has fixed costs. 1999 x 2112 x 7168 (FP32, accumulated): 144 tiles of 256 52 us, 272 of 128 56.
     // Groups of few rows read their weights at HBM rate, and tiles of 128 leave a shorter last wave: 32 groups of 24 rows, 256 -> 128 wide:
-    // N 7168, K 2048 89 -> 84 us, N 4096, K 7168 161 -> 154; 64 of 8 rows, N 4096, K 4096 169 -> 171.
+    // N 7168, K 2048 89 -> 84 us, N 4096, K 7168 161 -> 154; 64 of 8 rows, N 4096, K 4096 169 -> 171. Tile width and loads of 32 rows (below)
+    // together, masked buffers of 256 rows, 32 groups, without -> with: N 4096, K 7168 8 rows 165 -> 152, 24 174 -> 152, 48 179 -> 162, 96
+    // 183 -> 175; N 7168, K 2048 48 rows 99 -> 86, 96 102 -> 92. Past the bound it would still serve one tile of rows (112 rows 184 -> 173 and
+    // 107 -> 96, 128 rows 183 -> 177 and 106 -> 103) and lose with two (160 rows 316 -> 340 and 149 -> 176, 192 rows 309 -> 357).
+    // With psum the host knows the buffer's rows only: a plan's buffer of alignment 128 is not taken for one of few rows.
     const bool few_rows = (masked || psum) && expected <= 96;
     int block_n = 256;
     if (tuning().block_n != 0) {
@@ -189,7 +193,9 @@ int run_block_scaled_gemm(const dgb200_fp8_block_scaled_gemm_args& a, cudaStream
     }
     // Pairs load 32 KB per SM and K block instead of 48. Single CTAs -> pairs (us): dense 4096 x 4096 x 7168 116 -> 111, 8192 x 7168 x 4096
     // 228 -> 216. With groups half a pair tile is lost on every second one: N 4096, K 7168, 32 groups of 247 rows 323 -> 371, 8 of
-    // 900 239 -> 250, 4 of 2000 248 -> 250.
+    // 900 239 -> 250. Above the bound, in turn, 4 groups: N 4096, K 7168 2100 rows 286 -> 284, 2500 333 -> 321, 4000 508 -> 488, 6000 737 ->
+    // 712; N 7168, K 2048 170 -> 178, 166 -> 159, 292 -> 284, 433 -> 431 (2100 rows are 17 tiles of 128 but 9 of 256). Below it groups that
+    // fill their last pair tile would gain as much (1000, 1500, 2000 rows: 2 to 4 %), but the host does not know the groups.
     const long long pair_tiles = groups * ((expected + 255) / 256) * ((a.n + 255) / 256);
     const bool pair = !row_ids && block_n == 256 && sms >= 2 && tuning().pair != 0 &&
                       (tuning().pair == 1 || (expected > (dense ? 128 : 2048) && pair_tiles * 2 >= sms));

@@ -13,7 +13,7 @@ namespace dgb {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxPlanExperts = 1024;
 
-// Experts counted per chunk of entries: chunk_hist[chunk][e].
+// Experts counted per chunk of entries: chunk_hist[chunk][e]. (The end of the last chunk, rounded up, stays below 2^31: the host sees to it.)
 __global__ void __launch_bounds__(kPlanThreads)
 dgb200_sort_count_kernel(const long long* __restrict__ topk_idx, int entries, int chunk_entries, int experts, int* __restrict__ chunk_hist) {
     pdl_prologue();
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(128) dgb200_unpermute_kernel(const UnpermutePa
 // The gradients of the weighted sum: d_rows[dest_row[t, k]] = weights[t, k] dy[t], d_weights[t, k] = <rows[dest_row[t, k]], dy[t]> (0 for a
 // masked entry); padding rows of d_rows = 0, as the K-grouped GEMM wants them, rows behind the last segment stay. One CTA per token: dy is
 // read once a batch of eight entries, the dot products are summed in a fixed order (thread, warp, CTA). HBM bounds it; with 76 registers
-// three CTAs a SM kept too little in flight (8192 tokens x 4096 x 8, forward and backward: 283 us, with four 275, its bytes at the copy
-// rate 272).
+// three CTAs a SM kept too little in flight (8192 tokens x 4096 x 8, forward and backward: 283 us, with four, which spill two words of the
+// BF16 form, 275, its bytes at the copy rate 272).
 template <typename T, int kVec>
 __global__ void __launch_bounds__(256, 4) dgb200_unpermute_backward_kernel(const UnpermuteParams p) {
     using V = RowVec<T, kVec>;

@@ -110,7 +110,8 @@ def m_grouped_fp8_fp4_gemm_nt_contiguous(a: Tuple[torch.Tensor, torch.Tensor], b
                                          use_psum_layout: bool = False, ensure_zero_padding: bool = True,
                                          expected_m_for_psum_layout: Optional[int] = None) -> None:
     """D[m] = A[m] @ B[group(m)].T; reference: m_grouped_fp8_fp4_gemm_nt_contiguous, csrc/apis/gemm.hpp:166-232.
-    float32 scales with ``disable_ue8m0_cast``: as in ``fp8_fp4_gemm_nt``."""
+    float32 scales with ``disable_ue8m0_cast``: as in ``fp8_fp4_gemm_nt``; the scales of padding rows are not read (``ensure_zero_padding``
+    stores zeros there unless a holds NaN). ``expected_m_for_psum_layout`` is accepted and steers nothing here."""
     del compiled_dims
     a_q, a_sf = a
     b_q, b_sf = b

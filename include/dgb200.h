@@ -42,7 +42,7 @@ int dgb200_get_num_sms(void);
 /* Process-wide tuning knobs of the GEMM kernels. Plays the role of the reference's heuristics overrides
  * (csrc/apis/runtime.hpp:21-41).
  *   "block_n"            0 = automatic, 128 or 256: width of an output tile of the tokens-on-M kernel and of the FP8 GEMM with FP32 scales
- *                        (which also has 64 and 32, and with a width given does not split K).
+ *                        (which with a width given does not split K; the widths 64 and 32 that it takes by itself cannot be set).
  *   "swap_ab"            layer GEMMs: -1 = choose the tile orientation from the expected rows per expert (default:
  *                        swapped-operand kernel alone for decode-sized batches, experts split by size around 128
  *                        rows per expert, tokens-on-M kernel otherwise), 0 = tokens-on-M kernel only, 1 = everything
@@ -469,7 +469,8 @@ int dgb200_moe_dispatch_plan_noalloc(const int64_t* topk_idx, int32_t num_tokens
 /* FP8 GEMM whose operands carry an FP32 scale per block of 128 (any positive value, not only powers of two):
  *   d[m, n] = c[m, n] + sum over K blocks kb of sfa[m, kb] * sfb[n / 128, kb] * sum_{k in kb} a[m, k] * b[n, k]
  * The products of one K block are summed by the tensor core in FP32, the K blocks by FP32 multiply-adds with the (rounded) product of
- * the two scales, in ascending order. The form the reference's GEMMs take with FP32 scales and disable_ue8m0_cast
+ * the two scales, in ascending order; a dense GEMM with a long K and few tiles sums parts of K so and then the parts, in ascending order
+ * too (never with the knob "split_k" at 0). The form the reference's GEMMs take with FP32 scales and disable_ue8m0_cast
  * (csrc/apis/gemm.hpp:73-124, :166-297), which it builds for the previous architecture only.
  *   a    e4m3 [m, k] (masked: [num_groups, m, k]), K-major, rows dense.
  *   sfa  scale of row r and K block kb (of group g, masked only) at sfa[g * sfa_group_stride + r * sfa_row_stride + kb * sfa_k_stride].
