@@ -171,3 +171,24 @@ def test_the_plan_with_the_most_chunks(dg):
         want[kept] = start[flat[kept]] + torch.arange(kept.numel(), device='cuda') - first[flat[kept]]
         assert torch.equal(plan.dest_row.flatten().long(), want)
         assert torch.equal(plan.expert_start.long(), start) and torch.equal(plan.expert_end.long(), start + counts)
+
+
+@pytest.mark.parametrize('rows, inter', [(7, 264), (2500, 2048)])
+def test_rows_beside_special_ones_keep_their_bits(dg, rows, inter):
+    """NaN, infinities, far gates and products near the end of FP32 in some rows: the others' codes and scales are what they are without."""
+    g = torch.Generator(device='cuda').manual_seed(7)
+    x = (torch.randn(rows, 2 * inter, generator=g, device='cuda') * 2).bfloat16()
+    q, sf = dg.swiglu_per_token_cast_to_fp8(x)
+    special = x.clone()
+    for row, (gate, up) in zip(range(1, rows, 2), ((float('nan'), 1.0), (-100.0, 1e36), (1e19, 2e19))):
+        special[row, 3], special[row, inter + 3] = gate, up
+    changed = [r for r in range(1, rows, 2)][:3]
+    got_q, got_sf = dg.swiglu_per_token_cast_to_fp8(special)
+    kept = torch.ones(rows, dtype=torch.bool, device='cuda')
+    kept[changed] = False
+    assert torch.equal(got_q.view(torch.uint8)[kept], q.view(torch.uint8)[kept]) and torch.equal(got_sf[kept], sf[kept])
+    assert torch.equal(got_q.view(torch.uint8)[:, 128:], q.view(torch.uint8)[:, 128:]) and torch.equal(got_sf[:, 1:], sf[:, 1:])
+    assert torch.isnan(got_q.float()[1, 3]) and torch.isfinite(got_q.float()[2:]).all() and torch.isfinite(got_sf).all()
+    # 1e19 and 2e19: the product is finite, four times it is not
+    product = special[5, 3].double() * special[5, inter + 3].double()
+    assert abs(float(got_sf[5, 0]) / float(product / 448) - 1) <= 2.0 ** -20 and float(got_q.float()[5, 3]) == 448
